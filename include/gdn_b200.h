@@ -189,6 +189,57 @@ int gdn_wy_prep_sm100(const gdn_fwd_args* args, float* W, float* U, void* stream
  */
 int gdn_selftest_wait_timeout(int* status, long long limit_cycles, void* stream);
 
+/*
+ * Gated linear recurrence, one chain per channel (c = one of H*D):
+ *
+ *     h_t = a_t h_{t-1} + x_t,  o_t = h_t,  a_t = exp(g_t)
+ *                               (sigmoid(g_t) with GDN_FLAG_G_LOGSIGMOID)
+ *
+ *   x   [B, T, H, D]  x_dtype               (last dim contiguous)
+ *   g   [B, T, H, D]  GDN_DTYPE_F32 or x_dtype: log decays (<= 0) or logits
+ *   h0  [B, H, D]     float32 contiguous, or NULL for a zero state
+ *   o   [B, T, H, D]  GDN_DTYPE_F32 or x_dtype (last dim contiguous)
+ *   ht  [B, H, D]     float32 contiguous, or NULL; may be h0 (in place)
+ *   states            float32, gdn_gated_scan_states_bytes() bytes, or NULL:
+ *                     written by the forward, needed by the backward
+ * Strides are in elements, for (b, t, h), and not negative.  Any D, any T >= 1
+ * and any strides are taken; rows of four aligned elements run fastest.
+ *
+ * The backward reads x, g, states and, where not NULL, d_o [B, T, H, D] in
+ * o_dtype (the gradient of o) and dht [B, H, D] float32; it writes dx (x_dtype),
+ * dg (g_dtype) and, where not NULL, dh0 [B, H, D] float32.
+ */
+typedef struct gdn_gated_scan_args {
+  int32_t abi_version; /* must be GDN_B200_ABI_VERSION */
+  int32_t B, T, H, D;
+  int32_t x_dtype, g_dtype, o_dtype;
+  int32_t flags; /* GDN_FLAG_G_LOGSIGMOID or 0 */
+  int32_t reserved;
+  const void* x;
+  int64_t x_stride[3];
+  const void* g;
+  int64_t g_stride[3];
+  const float* h0;
+  void* o;
+  int64_t o_stride[3];
+  float* ht;
+  float* states;
+  const void* d_o;
+  int64_t do_stride[3];
+  const float* dht;
+  void* dx;
+  int64_t dx_stride[3];
+  void* dg;
+  int64_t dg_stride[3];
+  float* dh0;
+} gdn_gated_scan_args;
+
+int gdn_gated_scan_fwd_sm100(const gdn_gated_scan_args* args, void* stream);
+int gdn_gated_scan_bwd_sm100(const gdn_gated_scan_args* args, void* stream);
+
+/* Bytes of `states` for these sizes and this x_dtype; 0 for invalid arguments. */
+uint64_t gdn_gated_scan_states_bytes(const gdn_gated_scan_args* args);
+
 /* Human-readable text of a gdn_status code. */
 const char* gdn_status_string(int code);
 

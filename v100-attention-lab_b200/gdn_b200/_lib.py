@@ -41,6 +41,7 @@ WORKSPACE_HEADER_BYTES = 256  # the prep's item counter, ahead of the state area
 
 # Every symbol include/gdn_b200.h declares.
 EXPORTED_SYMBOLS = ("gdn_fwd_sm100", "gdn_fwd_sm100_noalloc", "gdn_fwd_workspace_bytes", "gdn_wy_prep_sm100",
+                    "gdn_gated_scan_fwd_sm100", "gdn_gated_scan_bwd_sm100", "gdn_gated_scan_states_bytes",
                     "gdn_selftest_wait_timeout", "gdn_status_string", "gdn_abi_version")
 
 _i64x3 = ctypes.c_int64 * 3
@@ -82,6 +83,31 @@ class GdnFwdArgs(ctypes.Structure):
     ]
 
 
+class GatedScanArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_gated_scan_args`` (include/gdn_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "B", "T", "H", "D", "x_dtype", "g_dtype", "o_dtype",
+                                              "flags", "reserved")] + [
+        ("x", ctypes.c_void_p),
+        ("x_stride", _i64x3),
+        ("g", ctypes.c_void_p),
+        ("g_stride", _i64x3),
+        ("h0", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("o_stride", _i64x3),
+        ("ht", ctypes.c_void_p),
+        ("states", ctypes.c_void_p),
+        ("d_o", ctypes.c_void_p),
+        ("do_stride", _i64x3),
+        ("dht", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("dx_stride", _i64x3),
+        ("dg", ctypes.c_void_p),
+        ("dg_stride", _i64x3),
+        ("dh0", ctypes.c_void_p),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -117,6 +143,11 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
         lib.gdn_wy_prep_sm100.argtypes = [ctypes.POINTER(GdnFwdArgs), ctypes.c_void_p, ctypes.c_void_p,
                                           ctypes.c_void_p]
         lib.gdn_wy_prep_sm100.restype = ctypes.c_int
+        for name in ("gdn_gated_scan_fwd_sm100", "gdn_gated_scan_bwd_sm100"):
+            getattr(lib, name).argtypes = [ctypes.POINTER(GatedScanArgs), ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
+        lib.gdn_gated_scan_states_bytes.argtypes = [ctypes.POINTER(GatedScanArgs)]
+        lib.gdn_gated_scan_states_bytes.restype = ctypes.c_uint64
         lib.gdn_selftest_wait_timeout.argtypes = [ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]
         lib.gdn_selftest_wait_timeout.restype = ctypes.c_int
         lib.gdn_status_string.argtypes = [ctypes.c_int]

@@ -316,6 +316,18 @@ def gdn_wy_prep(q, k, v, beta, g, chunk_size=64, check=True):
     return W, U
 
 
+def _launch(fn, where: str, args, dev: torch.device):
+    """Call a C entry point on ``dev``'s current stream; raise on its status."""
+    idx = dev.index
+    if idx == torch.cuda.current_device():
+        rc = fn(ctypes.byref(args), torch.cuda.current_stream(idx).cuda_stream)
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(ctypes.byref(args), torch.cuda.current_stream(idx).cuda_stream)
+    if rc != _lib.OK:
+        _raise(rc, where)
+
+
 def _raise(rc: int, where: str):
     if rc in (_lib.ERR_INVALID_ARGUMENT, _lib.ERR_ALIGNMENT):
         raise ValueError(f"{where}: {_lib.status_string(rc)}")
