@@ -240,6 +240,108 @@ int gdn_gated_scan_bwd_sm100(const gdn_gated_scan_args* args, void* stream);
 /* Bytes of `states` for these sizes and this x_dtype; 0 for invalid arguments. */
 uint64_t gdn_gated_scan_states_bytes(const gdn_gated_scan_args* args);
 
+/*
+ * Causal attention over a sliding window and the first tokens (sinks).  Query
+ * row i sits at position p = S - T + i and sees key j when
+ *     j <= p,  j < lengths[b],  and  (p - j < window  or  j < sinks).
+ * o = softmax(scale q k^T) v over the visible keys; 0 where there are none
+ * (rows at or behind their sequence's length).  Hidden keys and values may hold
+ * anything, NaN and infinities included.
+ *   q, o  [B, T, H, D]   k, v  [B, S, HK, D]   fp16 or bf16, D = 64 or 128,
+ *         T <= S, H a multiple of HK (query head h reads key head h / (H / HK))
+ *   lengths  [B] int32 on the device, clamped to 0..S, or NULL (all S)
+ * Strides in elements for (batch, row, head); bases and strides 16-byte aligned.
+ */
+typedef struct gdn_window_attn_args {
+  int32_t abi_version; /* must be GDN_B200_ABI_VERSION */
+  int32_t B, T, S, H, HK, D;
+  int32_t dtype;
+  int32_t window, sinks;
+  float scale; /* > 0 */
+  int32_t reserved;
+  const void* q;
+  int64_t q_stride[3];
+  const void* k;
+  int64_t k_stride[3];
+  const void* v;
+  int64_t v_stride[3];
+  void* o;
+  int64_t o_stride[3];
+  const int32_t* lengths;
+  int32_t* status; /* optional device int; the kernel ORs error bits into it */
+} gdn_window_attn_args;
+
+int gdn_window_attn_sm100(const gdn_window_attn_args* args, void* stream);
+
+/*
+ * One token of the windowed attention against a ring cache: the token at
+ * positions[b] (0 for a sequence's first) is written into its slot and attends
+ * to itself, the window - 1 tokens before it and the first `sinks` ones.
+ *   slot(j) = j                                             for j < capacity
+ *             sinks + (j - sinks) mod (capacity - sinks)    otherwise
+ * positions[b] < 0: the row is off, o is 0 and the cache is left as it is.
+ * Slots that hold no visible token may hold anything, NaN included.
+ *   q, o  [B, H, D]   k, v  [B, HK, D]   k_cache, v_cache  [B, capacity, HK, D]
+ *   positions  [B] int32 on the device;  capacity >= window + sinks
+ * Strides in elements, (batch, head) and (batch, slot, head); 16-byte aligned.
+ * The caches must not overlap each other, nor any sequence's those of another.
+ */
+typedef struct gdn_window_step_args {
+  int32_t abi_version; /* must be GDN_B200_ABI_VERSION */
+  int32_t B, H, HK, D;
+  int32_t capacity, window, sinks;
+  int32_t dtype;
+  float scale; /* > 0 */
+  const void* q;
+  int64_t q_stride[2];
+  const void* k;
+  int64_t k_stride[2];
+  const void* v;
+  int64_t v_stride[2];
+  void* k_cache;
+  int64_t kc_stride[3];
+  void* v_cache;
+  int64_t vc_stride[3];
+  void* o;
+  int64_t o_stride[2];
+  const int32_t* positions;
+} gdn_window_step_args;
+
+int gdn_window_step_sm100(const gdn_window_step_args* args, void* stream);
+
+/*
+ * One token of the Gated DeltaNet recurrence of gdn_fwd_sm100 (gdn_ref.py:28-45
+ * for T = 1): the state [B, H, V, K] float32, contiguous, is updated in place.
+ *   q, k [B, H, K]   v [B, H, V]   in_dtype (fp16 or bf16, last dim contiguous,
+ *   8-byte aligned rows);  beta, g [B, H] float32, g may be NULL (g == 0);
+ *   o [B, H, V] out_dtype
+ * Strides in elements for (b, h); flags and scale as in gdn_fwd_args, without
+ * the solver flags.
+ */
+typedef struct gdn_step_args {
+  int32_t abi_version; /* must be GDN_B200_ABI_VERSION */
+  int32_t B, H, K, V;
+  int32_t in_dtype, out_dtype;
+  int32_t flags;
+  float scale;
+  int32_t reserved;
+  const void* q;
+  int64_t q_stride[2];
+  const void* k;
+  int64_t k_stride[2];
+  const void* v;
+  int64_t v_stride[2];
+  const float* beta;
+  int64_t beta_stride[2];
+  const float* g;
+  int64_t g_stride[2];
+  float* state;
+  void* o;
+  int64_t o_stride[2];
+} gdn_step_args;
+
+int gdn_step_sm100(const gdn_step_args* args, void* stream);
+
 /* Human-readable text of a gdn_status code. */
 const char* gdn_status_string(int code);
 

@@ -1,0 +1,184 @@
+// One token of the Gated DeltaNet recurrence, the state updated in place:
+//
+//     h <- e^g h;   u = beta (v - h k);   h <- h + u k^T;   o = scale h q
+//
+// per (batch, head), h the V x K state.  Memory bounds it: 64 KB of state are
+// read and written per head.  The rows of h are independent, so a warp takes 8
+// of them (4 KB): each lane holds 4 columns of every row, both dot products
+// of all rows (h k and h q, from the decayed state) are summed over the warp in
+// one butterfly of 16 values (16 + 1 shuffles), and the output follows from them as
+// h' q = h q + u (k . q), without another sum over the new state.
+#include "../../include/gdn_b200.h"
+#include "host_util.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+
+namespace gdn {
+namespace gs {
+namespace {
+
+constexpr int kN = 128;     // K = V
+constexpr int kRows = 8;    // state rows per warp
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+
+struct Params {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* beta;
+  const float* g;
+  float* state;
+  void* o;
+  long long qs[2], ks[2], vs[2], bs[2], gs[2], os[2];  // (b, h)
+  int H;
+  int flags;
+  float scale;
+};
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  union {
+    uint2 r;
+    T e[4];
+  } u;
+  u.r = *reinterpret_cast<const uint2*>(p);
+  return make_float4(float(u.e[0]), float(u.e[1]), float(u.e[2]), float(u.e[3]));
+}
+
+template <typename T, typename OT>
+__global__ void __launch_bounds__(kThreads) gdn_step_kernel(const Params P) {
+  const int bh = blockIdx.x, b = bh / P.H, h = bh - b * P.H;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = (blockIdx.y * kWarps + warp) * kRows;
+  float4* st = reinterpret_cast<float4*>(P.state + (long long)bh * kN * kN + row0 * kN) + lane;
+  float4 s[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) s[r] = st[r * (kN / 4)];
+  float4 k = load4(static_cast<const T*>(P.k) + P.ks[0] * b + P.ks[1] * h + lane * 4);
+  float4 q = load4(static_cast<const T*>(P.q) + P.qs[0] * b + P.qs[1] * h + lane * 4);
+  const int mine = (lane >> 1) & 7;  // the row whose sums this lane ends up with
+  const float v = float(static_cast<const T*>(P.v)[P.vs[0] * b + P.vs[1] * h + row0 + mine]);
+  float beta = P.beta[P.bs[0] * b + P.bs[1] * h];
+  if (P.flags & GDN_FLAG_BETA_SIGMOID) beta = 1.f / (1.f + expf(-beta));
+  float a = 1.f;
+  if (P.g != nullptr) {
+    const float g = P.g[P.gs[0] * b + P.gs[1] * h];
+    a = (P.flags & GDN_FLAG_G_LOGSIGMOID) ? 1.f / (1.f + expf(-g)) : expf(g);
+  }
+  float kq = k.x * q.x + k.y * q.y + k.z * q.z + k.w * q.w;
+  if (P.flags & GDN_FLAG_QK_L2NORM) {
+    const float nk = rsqrtf(warp_sum(k.x * k.x + k.y * k.y + k.z * k.z + k.w * k.w) + 1e-6f);
+    const float nq = rsqrtf(warp_sum(q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w) + 1e-6f);
+    k = make_float4(k.x * nk, k.y * nk, k.z * nk, k.w * nk);
+    q = make_float4(q.x * nq, q.y * nq, q.z * nq, q.w * nq);
+    kq = k.x * q.x + k.y * q.y + k.z * q.z + k.w * q.w;
+  }
+  kq = warp_sum(kq);
+  float d[2 * kRows];  // h k of the rows, then h q
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    s[r] = make_float4(a * s[r].x, a * s[r].y, a * s[r].z, a * s[r].w);
+    d[r] = s[r].x * k.x + s[r].y * k.y + s[r].z * k.z + s[r].w * k.w;
+    d[kRows + r] = s[r].x * q.x + s[r].y * q.y + s[r].z * q.z + s[r].w * q.w;
+  }
+  // Halving butterfly: after it lane L holds value 8 (L >> 4) + ((L >> 1) & 7).
+#pragma unroll
+  for (int n = kRows, x = 16; n >= 1; n >>= 1, x >>= 1) {
+    const bool up = lane & x;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float give = up ? d[i] : d[i + n], keep = up ? d[i + n] : d[i];
+      d[i] = keep + __shfl_xor_sync(0xffffffffu, give, x);
+    }
+  }
+  d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
+  const float u_mine = beta * (v - d[0]);  // right in the lower half-warp, which holds h k
+  const float u_low = __shfl_sync(0xffffffffu, u_mine, lane & 15);
+  if (lane >= 16 && !(lane & 1)) {
+    const float o = P.scale * fmaf(u_low, kq, d[0]);
+    static_cast<OT*>(P.o)[P.os[0] * b + P.os[1] * h + row0 + mine] = OT(o);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const float u = __shfl_sync(0xffffffffu, u_mine, 2 * r);
+    st[r * (kN / 4)] = make_float4(fmaf(u, k.x, s[r].x), fmaf(u, k.y, s[r].y), fmaf(u, k.z, s[r].z), fmaf(u, k.w, s[r].w));
+  }
+}
+
+// ------------------------------------------------------------------ host side
+int validate(const gdn_step_args* a) {
+  if (a == nullptr || a->abi_version != GDN_B200_ABI_VERSION) return GDN_ERR_INVALID_ARGUMENT;
+  if (a->B < 1 || a->H < 1 || a->K < 1 || a->V < 1) return GDN_ERR_INVALID_ARGUMENT;
+  if (a->flags & ~(GDN_FLAG_QK_L2NORM | GDN_FLAG_BETA_SIGMOID | GDN_FLAG_G_LOGSIGMOID)) return GDN_ERR_INVALID_ARGUMENT;
+  if (!(a->scale == a->scale) || a->scale > 3.0e38f || a->scale < -3.0e38f) return GDN_ERR_INVALID_ARGUMENT;
+  if (a->in_dtype != GDN_DTYPE_F16 && a->in_dtype != GDN_DTYPE_BF16)
+    return a->in_dtype == GDN_DTYPE_F32 ? GDN_ERR_UNSUPPORTED : GDN_ERR_INVALID_ARGUMENT;
+  if (a->out_dtype != GDN_DTYPE_F32 && a->out_dtype != GDN_DTYPE_F16 && a->out_dtype != GDN_DTYPE_BF16)
+    return GDN_ERR_INVALID_ARGUMENT;
+  if (!a->q || !a->k || !a->v || !a->beta || !a->state || !a->o) return GDN_ERR_INVALID_ARGUMENT;
+  if (a->K != kN || a->V != kN || (long long)a->B * a->H > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED;
+  if (reinterpret_cast<uintptr_t>(a->state) % 16 || reinterpret_cast<uintptr_t>(a->beta) % 4 ||
+      reinterpret_cast<uintptr_t>(a->g) % 4)
+    return GDN_ERR_ALIGNMENT;
+  const void* ptr[3] = {a->q, a->k, a->v};
+  const int64_t* st[3] = {a->q_stride, a->k_stride, a->v_stride};
+  for (int i = 0; i < 3; ++i) {
+    if (reinterpret_cast<uintptr_t>(ptr[i]) % 8) return GDN_ERR_ALIGNMENT;
+    for (int j = 0; j < 2; ++j)
+      if (st[i][j] < 0 || st[i][j] % 4) return GDN_ERR_ALIGNMENT;
+  }
+  if (reinterpret_cast<uintptr_t>(a->o) % size_t(dtype_size(a->out_dtype))) return GDN_ERR_ALIGNMENT;
+  for (int j = 0; j < 2; ++j)
+    if (a->o_stride[j] < 0 || a->beta_stride[j] < 0 || a->g_stride[j] < 0) return GDN_ERR_INVALID_ARGUMENT;
+  return GDN_OK;
+}
+
+template <typename T>
+int launch(const Params& p, int out_dtype, int bh, cudaStream_t s) {
+  const dim3 grid(bh, kN / (kRows * kWarps));
+  switch (out_dtype) {
+    case GDN_DTYPE_F32: gdn_step_kernel<T, float><<<grid, kThreads, 0, s>>>(p); break;
+    case GDN_DTYPE_F16: gdn_step_kernel<T, __half><<<grid, kThreads, 0, s>>>(p); break;
+    default: gdn_step_kernel<T, __nv_bfloat16><<<grid, kThreads, 0, s>>>(p); break;
+  }
+  return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
+}
+
+int run(const gdn_step_args* a, void* stream) {
+  const int rc = validate(a);
+  if (rc != GDN_OK) return rc;
+  int dev = 0;
+  if (!device_is_sm100(&dev)) return GDN_ERR_NO_DEVICE;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.q = a->q, p.k = a->k, p.v = a->v, p.beta = a->beta, p.g = a->g, p.state = a->state, p.o = a->o;
+  for (int j = 0; j < 2; ++j) {
+    p.qs[j] = a->q_stride[j], p.ks[j] = a->k_stride[j], p.vs[j] = a->v_stride[j];
+    p.bs[j] = a->beta_stride[j], p.gs[j] = a->g_stride[j], p.os[j] = a->o_stride[j];
+  }
+  p.H = a->H;
+  p.flags = a->flags;
+  p.scale = a->scale == 0.f ? 1.f : a->scale;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int bh = a->B * a->H;
+  return a->in_dtype == GDN_DTYPE_BF16 ? launch<__nv_bfloat16>(p, a->out_dtype, bh, s)
+                                       : launch<__half>(p, a->out_dtype, bh, s);
+}
+
+}  // namespace
+}  // namespace gs
+}  // namespace gdn
+
+extern "C" int gdn_step_sm100(const gdn_step_args* args, void* stream) { return gdn::gs::run(args, stream); }

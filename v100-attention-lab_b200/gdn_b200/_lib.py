@@ -42,9 +42,11 @@ WORKSPACE_HEADER_BYTES = 256  # the prep's item counter, ahead of the state area
 # Every symbol include/gdn_b200.h declares.
 EXPORTED_SYMBOLS = ("gdn_fwd_sm100", "gdn_fwd_sm100_noalloc", "gdn_fwd_workspace_bytes", "gdn_wy_prep_sm100",
                     "gdn_gated_scan_fwd_sm100", "gdn_gated_scan_bwd_sm100", "gdn_gated_scan_states_bytes",
+                    "gdn_window_attn_sm100", "gdn_window_step_sm100", "gdn_step_sm100",
                     "gdn_selftest_wait_timeout", "gdn_status_string", "gdn_abi_version")
 
 _i64x3 = ctypes.c_int64 * 3
+_i64x2 = ctypes.c_int64 * 2
 
 
 class GdnFwdArgs(ctypes.Structure):
@@ -108,6 +110,71 @@ class GatedScanArgs(ctypes.Structure):
     ]
 
 
+class WindowAttnArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_window_attn_args`` (include/gdn_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "B", "T", "S", "H", "HK", "D", "dtype", "window",
+                                              "sinks")] + [
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_stride", _i64x3),
+        ("k", ctypes.c_void_p),
+        ("k_stride", _i64x3),
+        ("v", ctypes.c_void_p),
+        ("v_stride", _i64x3),
+        ("o", ctypes.c_void_p),
+        ("o_stride", _i64x3),
+        ("lengths", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class WindowStepArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_window_step_args`` (include/gdn_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "B", "H", "HK", "D", "capacity", "window", "sinks",
+                                              "dtype")] + [
+        ("scale", ctypes.c_float),
+        ("q", ctypes.c_void_p),
+        ("q_stride", _i64x2),
+        ("k", ctypes.c_void_p),
+        ("k_stride", _i64x2),
+        ("v", ctypes.c_void_p),
+        ("v_stride", _i64x2),
+        ("k_cache", ctypes.c_void_p),
+        ("kc_stride", _i64x3),
+        ("v_cache", ctypes.c_void_p),
+        ("vc_stride", _i64x3),
+        ("o", ctypes.c_void_p),
+        ("o_stride", _i64x2),
+        ("positions", ctypes.c_void_p),
+    ]
+
+
+class StepArgs(ctypes.Structure):
+    """Mirror of ``struct gdn_step_args`` (include/gdn_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "B", "H", "K", "V", "in_dtype", "out_dtype",
+                                              "flags")] + [
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_stride", _i64x2),
+        ("k", ctypes.c_void_p),
+        ("k_stride", _i64x2),
+        ("v", ctypes.c_void_p),
+        ("v_stride", _i64x2),
+        ("beta", ctypes.c_void_p),
+        ("beta_stride", _i64x2),
+        ("g", ctypes.c_void_p),
+        ("g_stride", _i64x2),
+        ("state", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("o_stride", _i64x2),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -145,6 +212,10 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
         lib.gdn_wy_prep_sm100.restype = ctypes.c_int
         for name in ("gdn_gated_scan_fwd_sm100", "gdn_gated_scan_bwd_sm100"):
             getattr(lib, name).argtypes = [ctypes.POINTER(GatedScanArgs), ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
+        for name, args in (("gdn_window_attn_sm100", WindowAttnArgs), ("gdn_window_step_sm100", WindowStepArgs),
+                           ("gdn_step_sm100", StepArgs)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
             getattr(lib, name).restype = ctypes.c_int
         lib.gdn_gated_scan_states_bytes.argtypes = [ctypes.POINTER(GatedScanArgs)]
         lib.gdn_gated_scan_states_bytes.restype = ctypes.c_uint64

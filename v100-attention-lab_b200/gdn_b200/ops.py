@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["gdn_chunk_fwd", "gdn_chunk_fwd_v2", "gdn_wy_prep", "GdnError", "check_status"]
+__all__ = ["gdn_chunk_fwd", "gdn_chunk_fwd_v2", "gdn_step", "gdn_wy_prep", "GdnError", "check_status"]
 
 
 class GdnError(RuntimeError):
@@ -286,6 +286,82 @@ def gdn_chunk_fwd_fixed(q, k, v, beta, g, C=32, BV=32, num_warps=4, num_stages=1
     """
     del num_warps, num_stages
     return gdn_chunk_fwd(q, k, v, beta, g, chunk_size=C, block_v=BV, **kw)
+
+
+def gdn_step(q, k, v, beta, g, state, *, scale=None, output_dtype=None, use_qk_l2norm_in_kernel=False,
+             beta_activation=None, g_activation=None):
+    """One token of the Gated DeltaNet recurrence, the state updated in place.
+
+    Continues ``gdn_chunk_fwd`` token by token from the state that it returns
+    (gdn_ref.py:28-45 for T = 1).
+
+    Args:
+        q, k: [B, H, K] fp16/bf16 (last dim contiguous, rows 8-byte aligned)
+        v: [B, H, V] same dtype; K = V = 128
+        beta, g: [B, H], cast to fp32 if needed; g is the log decay, None = 0
+        state: [B, H, V, K] fp32, contiguous; overwritten with the new state
+        scale, use_qk_l2norm_in_kernel, beta_activation, g_activation: as in
+            ``gdn_chunk_fwd``
+        output_dtype: dtype of o (default q.dtype)
+    Returns:
+        o [B, H, V]
+
+    For inference: tensors that require gradients are refused while gradients
+    are recorded.
+    """
+    tensors = {"q": q, "k": k, "v": v, "beta": beta, "g": g, "state": state}
+    if g is None:
+        del tensors["g"]
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+    if q.dim() != 3 or v.dim() != 3:
+        raise ValueError("q, k, v must be [B, H, K] / [B, H, V]")
+    B, H, K = q.shape
+    V = v.shape[-1]
+    for name, shape in (("k", (B, H, K)), ("v", (B, H, V)), ("beta", (B, H)), ("g", (B, H)), ("state", (B, H, V, K))):
+        if name in tensors and tuple(tensors[name].shape) != shape:
+            raise ValueError(f"{name} shape {tuple(tensors[name].shape)} != {shape}")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError(f"q, k, v must share a dtype (got {q.dtype}, {k.dtype}, {v.dtype})")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise NotImplementedError(f"gdn_b200 takes fp16 or bf16 q/k/v (got {q.dtype})")
+    for name in ("q", "k", "v"):
+        if tensors[name].stride(-1) != 1:
+            raise ValueError(f"{name} must have a contiguous last dimension")
+    if state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError("state must be a contiguous float32 tensor: it is updated in place")
+    out_dtype = q.dtype if output_dtype is None else output_dtype
+    if out_dtype not in _DTYPES:
+        raise ValueError(f"unsupported output_dtype {out_dtype}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors.values()):
+        raise NotImplementedError("gdn_step has no backward: call it under torch.no_grad()")
+    flags = _prep_flags(use_qk_l2norm_in_kernel, beta_activation, g_activation)
+    if g is None and g_activation is not None:
+        raise ValueError("g_activation needs a g tensor")
+    dev = q.device
+    for name, t in tensors.items():
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (got device {t.device})")
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, q is on {dev}")
+    beta = beta if beta.dtype == torch.float32 else beta.float()
+    g = g if (g is None or g.dtype == torch.float32) else g.float()
+    lib = _lib.load()
+    o = torch.empty(B, H, V, dtype=out_dtype, device=dev)
+    a = _lib.StepArgs()
+    a.abi_version = _lib.ABI_VERSION
+    a.B, a.H, a.K, a.V = B, H, K, V
+    a.in_dtype, a.out_dtype = _DTYPES[q.dtype], _DTYPES[out_dtype]
+    a.flags = flags
+    a.scale = 1.0 if scale is None else float(scale)
+    for name, t in (("q", q), ("k", k), ("v", v), ("beta", beta), ("g", g), ("o", o)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+            setattr(a, name + "_stride", t.stride()[:2])
+    a.state = state.data_ptr()
+    _launch(lib.gdn_step_sm100, "gdn_step_sm100", a, dev)
+    return o
 
 
 def gdn_wy_prep(q, k, v, beta, g, chunk_size=64, check=True):
