@@ -181,3 +181,19 @@ def gdn_struct(**kw):
 def test_gdn_step_entry_rejects(lib, field, value, expected):
     assert lib.gdn_step_sm100(ctypes.byref(gdn_struct(**{field: value})), None) == expected
     assert lib.gdn_step_sm100(None, None) == 1
+
+
+def test_packed_argument_formats_match_the_structs():
+    """The struct formats that the calls pack have the C structs' sizes and field offsets."""
+    from gdn_b200 import _lib
+    for fmt, cls in ((_lib.GATED_SCAN_ARGS, _lib.GatedScanArgs), (_lib.WINDOW_ATTN_ARGS, _lib.WindowAttnArgs),
+                     (_lib.WINDOW_STEP_ARGS, _lib.WindowStepArgs), (_lib.STEP_ARGS, _lib.StepArgs)):
+        assert fmt.size == ctypes.sizeof(cls)
+        n = sum(f[1]._length_ if hasattr(f[1], "_length_") else 1 for f in cls._fields_)
+        vals = list(range(1, n + 1))
+        back = cls.from_buffer_copy(fmt.pack(*vals))
+        flat = []
+        for name, _ in cls._fields_:
+            x = getattr(back, name)
+            flat += list(x) if hasattr(x, "__len__") else [x]
+        assert flat == vals

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 from . import _build
@@ -175,6 +176,14 @@ class StepArgs(ctypes.Structure):
     ]
 
 
+# The same structs as struct formats: one pack() fills a call's arguments
+# several times faster than setting ctypes fields, which counts for calls of
+# single tokens.  Native sizes and alignment; checked against the mirrors above.
+GATED_SCAN_ARGS = struct.Struct("@10iP3qP3qPP3qPPP3qPP3qP3qP")
+WINDOW_ATTN_ARGS = struct.Struct("@10ifiP3qP3qP3qP3qPP")
+WINDOW_STEP_ARGS = struct.Struct("@9ifP2qP2qP2qP3qP3qP2qP")
+STEP_ARGS = struct.Struct("@8ifiP2qP2qP2qP2qP2qPP2q")
+
 _lock = threading.Lock()
 _lib = None
 
@@ -186,6 +195,8 @@ def lib_path() -> str:
 def load(build_if_missing: bool = False) -> ctypes.CDLL:
     """Load the shared library (building it first if asked and possible)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -210,14 +221,12 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
         lib.gdn_wy_prep_sm100.argtypes = [ctypes.POINTER(GdnFwdArgs), ctypes.c_void_p, ctypes.c_void_p,
                                           ctypes.c_void_p]
         lib.gdn_wy_prep_sm100.restype = ctypes.c_int
-        for name in ("gdn_gated_scan_fwd_sm100", "gdn_gated_scan_bwd_sm100"):
-            getattr(lib, name).argtypes = [ctypes.POINTER(GatedScanArgs), ctypes.c_void_p]
+        # the argument struct as bytes (see the formats above) or by reference
+        for name in ("gdn_gated_scan_fwd_sm100", "gdn_gated_scan_bwd_sm100", "gdn_window_attn_sm100",
+                     "gdn_window_step_sm100", "gdn_step_sm100"):
+            getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
             getattr(lib, name).restype = ctypes.c_int
-        for name, args in (("gdn_window_attn_sm100", WindowAttnArgs), ("gdn_window_step_sm100", WindowStepArgs),
-                           ("gdn_step_sm100", StepArgs)):
-            getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
-            getattr(lib, name).restype = ctypes.c_int
-        lib.gdn_gated_scan_states_bytes.argtypes = [ctypes.POINTER(GatedScanArgs)]
+        lib.gdn_gated_scan_states_bytes.argtypes = [ctypes.c_void_p]
         lib.gdn_gated_scan_states_bytes.restype = ctypes.c_uint64
         lib.gdn_selftest_wait_timeout.argtypes = [ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]
         lib.gdn_selftest_wait_timeout.restype = ctypes.c_int

@@ -309,58 +309,55 @@ def gdn_step(q, k, v, beta, g, state, *, scale=None, output_dtype=None, use_qk_l
     For inference: tensors that require gradients are refused while gradients
     are recorded.
     """
-    tensors = {"q": q, "k": k, "v": v, "beta": beta, "g": g, "state": state}
-    if g is None:
-        del tensors["g"]
-    for name, t in tensors.items():
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
+    if not isinstance(q, torch.Tensor) or not isinstance(v, torch.Tensor):
+        raise TypeError("q and v must be torch.Tensors")
     if q.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k, v must be [B, H, K] / [B, H, V]")
     B, H, K = q.shape
-    V = v.shape[-1]
-    for name, shape in (("k", (B, H, K)), ("v", (B, H, V)), ("beta", (B, H)), ("g", (B, H)), ("state", (B, H, V, K))):
-        if name in tensors and tuple(tensors[name].shape) != shape:
-            raise ValueError(f"{name} shape {tuple(tensors[name].shape)} != {shape}")
-    if q.dtype != k.dtype or q.dtype != v.dtype:
-        raise ValueError(f"q, k, v must share a dtype (got {q.dtype}, {k.dtype}, {v.dtype})")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise NotImplementedError(f"gdn_b200 takes fp16 or bf16 q/k/v (got {q.dtype})")
-    for name in ("q", "k", "v"):
-        if tensors[name].stride(-1) != 1:
+    V = v.shape[2]
+    dev, dtype, bh = q.device, q.dtype, (B, H)
+    grad = torch.is_grad_enabled()
+    for name, t, shape in (("q", q, (B, H, K)), ("k", k, (B, H, K)), ("v", v, (B, H, V)), ("beta", beta, bh), ("g", g, bh),
+                           ("state", state, (B, H, V, K))):
+        if not isinstance(t, torch.Tensor):
+            if t is None and name == "g":
+                continue
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.shape != shape:
+            raise ValueError(f"{name} shape {tuple(t.shape)} != {shape}")
+        if grad and t.requires_grad:
+            raise NotImplementedError("gdn_step has no backward: call it under torch.no_grad()")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"q, k, v must share a dtype (got {dtype}, {k.dtype}, {v.dtype})")
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise NotImplementedError(f"gdn_b200 takes fp16 or bf16 q/k/v (got {dtype})")
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    for name, s in (("q", sq), ("k", sk), ("v", sv)):
+        if s[2] != 1:
             raise ValueError(f"{name} must have a contiguous last dimension")
     if state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError("state must be a contiguous float32 tensor: it is updated in place")
-    out_dtype = q.dtype if output_dtype is None else output_dtype
+    out_dtype = dtype if output_dtype is None else output_dtype
     if out_dtype not in _DTYPES:
         raise ValueError(f"unsupported output_dtype {out_dtype}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors.values()):
-        raise NotImplementedError("gdn_step has no backward: call it under torch.no_grad()")
     flags = _prep_flags(use_qk_l2norm_in_kernel, beta_activation, g_activation)
     if g is None and g_activation is not None:
         raise ValueError("g_activation needs a g tensor")
-    dev = q.device
-    for name, t in tensors.items():
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (got device {t.device})")
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, q is on {dev}")
-    beta = beta if beta.dtype == torch.float32 else beta.float()
-    g = g if (g is None or g.dtype == torch.float32) else g.float()
-    lib = _lib.load()
-    o = torch.empty(B, H, V, dtype=out_dtype, device=dev)
-    a = _lib.StepArgs()
-    a.abi_version = _lib.ABI_VERSION
-    a.B, a.H, a.K, a.V = B, H, K, V
-    a.in_dtype, a.out_dtype = _DTYPES[q.dtype], _DTYPES[out_dtype]
-    a.flags = flags
-    a.scale = 1.0 if scale is None else float(scale)
-    for name, t in (("q", q), ("k", k), ("v", v), ("beta", beta), ("g", g), ("o", o)):
+    for name, t in (("q", q), ("k", k), ("v", v), ("beta", beta), ("g", g), ("state", state)):
         if t is not None:
-            setattr(a, name, t.data_ptr())
-            setattr(a, name + "_stride", t.stride()[:2])
-    a.state = state.data_ptr()
-    _launch(lib.gdn_step_sm100, "gdn_step_sm100", a, dev)
+            _check_device(name, t, dev, "q")
+    if beta.dtype != torch.float32:
+        beta = beta.float()
+    if g is not None and g.dtype != torch.float32:
+        g = g.float()
+    o = torch.empty((B, H, V), dtype=out_dtype, device=dev)
+    sb, sg, so = beta.stride(), (0, 0) if g is None else g.stride(), o.stride()
+    args = _lib.STEP_ARGS.pack(
+        _lib.ABI_VERSION, B, H, K, V, _DTYPES[dtype], _DTYPES[out_dtype], flags, 1.0 if scale is None else float(scale), 0,
+        q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1],
+        beta.data_ptr(), sb[0], sb[1], 0 if g is None else g.data_ptr(), sg[0], sg[1],
+        state.data_ptr(), o.data_ptr(), so[0], so[1])
+    _launch(_lib.load().gdn_step_sm100, "gdn_step_sm100", args, dev)
     return o
 
 
@@ -392,14 +389,22 @@ def gdn_wy_prep(q, k, v, beta, g, chunk_size=64, check=True):
     return W, U
 
 
-def _launch(fn, where: str, args, dev: torch.device):
-    """Call a C entry point on ``dev``'s current stream; raise on its status."""
+def _check_device(name, t, dev, first):
+    """``t`` is a CUDA tensor on ``dev``, the device of the call's ``first`` tensor."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (got device {t.device})")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, {first} is on {dev}")
+
+
+def _launch(fn, where: str, args: bytes, dev: torch.device):
+    """Call a C entry point with a packed argument struct on ``dev``'s current stream; raise on its status."""
     idx = dev.index
     if idx == torch.cuda.current_device():
-        rc = fn(ctypes.byref(args), torch.cuda.current_stream(idx).cuda_stream)
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
-            rc = fn(ctypes.byref(args), torch.cuda.current_stream(idx).cuda_stream)
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(idx))
     if rc != _lib.OK:
         _raise(rc, where)
 

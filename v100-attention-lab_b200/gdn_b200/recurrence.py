@@ -8,12 +8,10 @@ in the sm_100a library through its C ABI.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _launch
+from .ops import _DTYPES, _check_device, _launch
 
 __all__ = ["gated_scan", "gated_scan_step"]
 
@@ -28,75 +26,62 @@ def _gate_flags(g_activation):
 
 def _check(x, g, state, state_name, output_dtype, dims):
     for name, t in (("x", x), ("g", g), (state_name, state)):
-        if t is not None and not isinstance(t, torch.Tensor):
+        if not isinstance(t, torch.Tensor) and (t is not None or name != "initial_state"):
             raise TypeError(f"{name} must be a torch.Tensor")
-    if x.dim() != len(dims):
-        raise ValueError(f"x must be [{', '.join(dims)}] (got shape {tuple(x.shape)})")
-    if g.shape != x.shape:
-        raise ValueError(f"g shape {tuple(g.shape)} != x shape {tuple(x.shape)}")
-    if 0 in x.shape:
-        raise ValueError(f"x must not be empty (got shape {tuple(x.shape)})")
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != len(dims):
+        raise ValueError(f"x must be [{', '.join(dims)}] (got shape {tuple(shape)})")
+    if g.shape != shape:
+        raise ValueError(f"g shape {tuple(g.shape)} != x shape {tuple(shape)}")
+    if 0 in shape:
+        raise ValueError(f"x must not be empty (got shape {tuple(shape)})")
     for name, t in (("x", x), ("g", g)):
         if t.dtype not in _DTYPES:
             raise NotImplementedError(f"{name} must be fp16, bf16 or fp32 (got {t.dtype})")
-        if t.stride(-1) != 1 and t.shape[-1] != 1:
+        if t.stride(-1) != 1 and shape[-1] != 1:
             raise ValueError(f"{name} must have a contiguous last dimension")
-    shape = (x.shape[0],) + tuple(x.shape[-2:])
-    if state is not None and tuple(state.shape) != shape:
-        raise ValueError(f"{state_name} must be [B, H, D] = {shape} (got {tuple(state.shape)})")
-    out_dtype = x.dtype if output_dtype is None else output_dtype
-    if out_dtype != x.dtype and out_dtype != torch.float32:
+    if state is not None and state.shape != (shape[0], shape[-2], shape[-1]):
+        raise ValueError(f"{state_name} must be [B, H, D] = {(shape[0], shape[-2], shape[-1])} (got {tuple(state.shape)})")
+    out_dtype = dtype if output_dtype is None else output_dtype
+    if out_dtype != dtype and out_dtype != torch.float32:
         raise ValueError(f"output_dtype must be x's dtype or torch.float32 (got {out_dtype})")
-    dev = x.device
     for name, t in (("x", x), ("g", g), (state_name, state)):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (got device {t.device})")
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, x is on {dev}")
+        if t is not None:
+            _check_device(name, t, x.device, "x")
     return out_dtype
 
 
-def _set(a, name, t):
-    """Pointer and (b, t, h) strides of a [B, T, H, D] tensor, or of a [B, H, D] one (T = 1)."""
-    st = t.stride()
-    setattr(a, name, t.data_ptr())
-    stride = (st[0], st[1], st[2]) if t.dim() == 4 else (st[0], 0, st[1])
-    setattr(a, ("do" if name == "d_o" else name) + "_stride", stride)
+def _at(t):
+    """Pointer and (b, t, h) strides of a [B, T, H, D] tensor, of a [B, H, D] one (T = 1) or of none."""
+    if t is None:
+        return 0, 0, 0, 0
+    s = t.stride()
+    return (t.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else (t.data_ptr(), s[0], 0, s[1])
 
 
-def _args(x, g, out_dtype, flags):
-    a = _lib.GatedScanArgs()
-    a.abi_version = _lib.ABI_VERSION
-    if x.dim() == 4:
-        a.B, a.T, a.H, a.D = x.shape
-    else:
-        a.B, a.H, a.D = x.shape
-        a.T = 1
-    a.x_dtype, a.g_dtype, a.o_dtype = _DTYPES[x.dtype], _DTYPES[g.dtype], _DTYPES[out_dtype]
-    a.flags = flags
-    _set(a, "x", x)
-    _set(a, "g", g)
-    return a
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _pack(x, g, o_dtype, flags, h0=None, o=None, ht=None, states=None, d_o=None, dht=None, dx=None, dg=None, dh0=None):
+    shape = x.shape
+    return _lib.GATED_SCAN_ARGS.pack(
+        _lib.ABI_VERSION, shape[0], shape[1] if len(shape) == 4 else 1, shape[-2], shape[-1],
+        _DTYPES[x.dtype], _DTYPES[g.dtype], _DTYPES[o_dtype], flags, 0,
+        *_at(x), *_at(g), _ptr(h0), *_at(o), _ptr(ht), _ptr(states), *_at(d_o), _ptr(dht), *_at(dx), *_at(dg), _ptr(dh0))
 
 
 def _forward(x, g, h0, flags, out_dtype, want_ht, want_states):
     lib = _lib.load()
-    dev = x.device
-    o = torch.empty(x.shape, dtype=out_dtype, device=dev)
-    a = _args(x, g, out_dtype, flags)
-    _set(a, "o", o)
-    ht = states = None
-    if h0 is not None:
-        a.h0 = h0.data_ptr()
-    if want_ht:
-        ht = torch.empty(x.shape[0], *x.shape[-2:], dtype=torch.float32, device=dev)
-        a.ht = ht.data_ptr()
+    dev, shape = x.device, x.shape
+    o = torch.empty(shape, dtype=out_dtype, device=dev)
+    ht = torch.empty((shape[0], shape[2], shape[3]), dtype=torch.float32, device=dev) if want_ht else None
+    states = None
     if want_states:
-        states = torch.empty(int(lib.gdn_gated_scan_states_bytes(ctypes.byref(a))) // 4, dtype=torch.float32, device=dev)
-        a.states = states.data_ptr()
-    _launch(lib.gdn_gated_scan_fwd_sm100, "gdn_gated_scan_fwd_sm100", a, dev)
+        nbytes = int(lib.gdn_gated_scan_states_bytes(_pack(x, g, out_dtype, flags)))
+        states = torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
+    _launch(lib.gdn_gated_scan_fwd_sm100, "gdn_gated_scan_fwd_sm100",
+            _pack(x, g, out_dtype, flags, h0=h0, o=o, ht=ht, states=states), dev)
     return o, ht, states
 
 
@@ -105,7 +90,7 @@ class _GatedScan(torch.autograd.Function):
     def forward(ctx, x, g, h0, flags, out_dtype, want_ht):
         o, ht, states = _forward(x, g, h0, flags, out_dtype, want_ht, True)
         ctx.save_for_backward(x, g, states)
-        ctx.flags, ctx.out_dtype, ctx.has_h0 = flags, out_dtype, h0 is not None
+        ctx.flags, ctx.out_dtype = flags, out_dtype
         ctx.set_materialize_grads(False)
         return o, ht
 
@@ -115,26 +100,17 @@ class _GatedScan(torch.autograd.Function):
         if d_o is None and dht is None:
             return None, None, None, None, None, None
         x, g, states = ctx.saved_tensors
-        lib = _lib.load()
-        a = _args(x, g, ctx.out_dtype, ctx.flags)
-        a.states = states.data_ptr()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         dg = torch.empty(g.shape, dtype=g.dtype, device=x.device)
-        _set(a, "dx", dx)
-        _set(a, "dg", dg)
-        dh0 = None
-        if d_o is not None:
-            if d_o.stride(-1) != 1:  # e.g. the expanded gradient of a sum
-                d_o = d_o.contiguous()
-            _set(a, "d_o", d_o)
+        need_x, need_g, need_h0 = ctx.needs_input_grad[:3]
+        dh0 = torch.empty((x.shape[0],) + x.shape[2:], dtype=torch.float32, device=x.device) if need_h0 else None
+        if d_o is not None and d_o.stride(-1) != 1:  # e.g. the expanded gradient of a sum
+            d_o = d_o.contiguous()
         if dht is not None:
             dht = dht.contiguous()
-            a.dht = dht.data_ptr()
-        if ctx.has_h0 and ctx.needs_input_grad[2]:
-            dh0 = torch.empty(x.shape[0], *x.shape[2:], dtype=torch.float32, device=x.device)
-            a.dh0 = dh0.data_ptr()
-        _launch(lib.gdn_gated_scan_bwd_sm100, "gdn_gated_scan_bwd_sm100", a, x.device)
-        return (dx if ctx.needs_input_grad[0] else None, dg if ctx.needs_input_grad[1] else None, dh0, None, None, None)
+        _launch(_lib.load().gdn_gated_scan_bwd_sm100, "gdn_gated_scan_bwd_sm100",
+                _pack(x, g, ctx.out_dtype, ctx.flags, states=states, d_o=d_o, dht=dht, dx=dx, dg=dg, dh0=dh0), x.device)
+        return dx if need_x else None, dg if need_g else None, dh0, None, None, None
 
 
 def gated_scan(x, g, initial_state=None, *, g_activation=None, output_dtype=None, output_final_state=True):
@@ -180,8 +156,6 @@ def gated_scan_step(x, g, state, *, g_activation=None, output_dtype=None):
     For inference: tensors that require gradients are refused while gradients
     are recorded.
     """
-    if state is None:
-        raise TypeError("state must be a torch.Tensor")
     out_dtype = _check(x, g, state, "state", output_dtype, ("B", "H", "D"))
     flags = _gate_flags(g_activation)
     if state.dtype != torch.float32 or not state.is_contiguous():
@@ -190,10 +164,7 @@ def gated_scan_step(x, g, state, *, g_activation=None, output_dtype=None):
         raise NotImplementedError("gated_scan_step has no backward: use gated_scan, or torch.no_grad()")
     if g.dtype != torch.float32 and g.dtype != x.dtype:
         g = g.float()
-    lib = _lib.load()
     o = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    a = _args(x, g, out_dtype, flags)
-    _set(a, "o", o)
-    a.h0 = a.ht = state.data_ptr()
-    _launch(lib.gdn_gated_scan_fwd_sm100, "gdn_gated_scan_fwd_sm100", a, x.device)
+    _launch(_lib.load().gdn_gated_scan_fwd_sm100, "gdn_gated_scan_fwd_sm100",
+            _pack(x, g, out_dtype, flags, h0=state, o=o, ht=state), x.device)
     return o
