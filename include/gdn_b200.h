@@ -203,7 +203,7 @@ int gdn_selftest_wait_timeout(int* status, long long limit_cycles, void* stream)
  *   states            float32, gdn_gated_scan_states_bytes() bytes, or NULL:
  *                     written by the forward, needed by the backward
  * Strides are in elements, for (b, t, h), and not negative.  Any D, any T >= 1
- * and any strides are taken; rows of four aligned elements run fastest.
+ * and any strides are taken; tensors whose rows are 16-byte aligned run fastest.
  *
  * The backward reads x, g, states and, where not NULL, d_o [B, T, H, D] in
  * o_dtype (the gradient of o) and dht [B, H, D] float32; it writes dx (x_dtype),
@@ -232,6 +232,7 @@ typedef struct gdn_gated_scan_args {
   void* dg;
   int64_t dg_stride[3];
   float* dh0;
+  int32_t* status; /* optional device int; the kernel ORs error bits into it */
 } gdn_gated_scan_args;
 
 int gdn_gated_scan_fwd_sm100(const gdn_gated_scan_args* args, void* stream);

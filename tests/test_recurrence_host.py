@@ -97,7 +97,7 @@ def test_backward_needs_its_buffers(lib):
 
 
 def test_states_bytes(lib):
-    # one fp32 row per tile: 64 rows of 16-bit x, 32 rows of fp32 x
-    assert lib.gdn_gated_scan_states_bytes(ctypes.byref(c_args(B=3, T=65))) == 3 * 2 * 16 * 4
-    assert lib.gdn_gated_scan_states_bytes(ctypes.byref(c_args(B=3, T=65, x_dtype=0))) == 3 * 3 * 16 * 4
+    # one fp32 row per tile: 128 rows of 16-bit x, 64 rows of fp32 x
+    assert lib.gdn_gated_scan_states_bytes(ctypes.byref(c_args(B=3, T=129))) == 3 * 2 * 16 * 4
+    assert lib.gdn_gated_scan_states_bytes(ctypes.byref(c_args(B=3, T=129, x_dtype=0))) == 3 * 3 * 16 * 4
     assert lib.gdn_gated_scan_states_bytes(ctypes.byref(c_args(T=0))) == 0

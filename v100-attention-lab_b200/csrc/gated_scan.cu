@@ -11,19 +11,26 @@
 // (A2, X2) after (A1, X1) is (A2 A1, A2 X1 + X2).  Memory bounds them: x and g
 // are read once and o is written once (dx and dg besides, in the backward).
 //
-// Split.  A chain's channels are the CTA's columns (32 lanes x V channels) and
-// its rows are split three ways: R consecutive rows per warp, held in
-// registers; 8 warps per CTA; up to 16 CTAs per cluster.  A cluster walks the
-// sequence in strides of S tiles.  Per stride every warp composes its rows,
-// the CTA composes its warps in shared memory and pushes its map to every CTA
-// of the cluster (distributed shared memory), and after one cluster barrier
-// each CTA folds the maps before its own into the running state, replays its
-// rows from registers and writes them.  The order of all sums is fixed, so
-// results repeat bit for bit; no CTA ever waits on global memory.
+// Split.  A CTA owns 64 channels (32 lanes x 2) and walks tiles of 128 rows;
+// consecutive tiles of a chain belong to the up to 16 CTAs of a cluster, which
+// advances in strides of that many tiles.  Per stride every warp composes its
+// rows, the CTA composes its warps in shared memory and sends its map to every
+// CTA of the cluster (distributed shared memory); each then folds the maps
+// before its own into the running state, replays its rows with the gates it
+// kept in registers, and writes them.  The order of all sums is fixed, so
+// results repeat bit for bit, and no CTA waits on global memory.
+//
+// Loads.  Tiles whose rows are 16-byte aligned come by TMA, issued by one
+// thread a stride ahead, while the current stride's maps are exchanged (copies
+// that each thread issued for itself took 40 % of the kernel's instructions;
+// bulk copies row by row were slower still).  Other tensors (odd sizes or
+// strides) take one channel per thread, each thread copying its own rows.
+// Rows beyond the sequence get x = 0 and a gate of exactly 1, which keeps the
+// arithmetic free of conditions.
 //
 // The backward walks the strides from the end.  It needs h_{t-1}; instead of
 // the rounded outputs it takes the fp32 state at each tile's start, which the
-// forward leaves behind (one row in 8 R), and recomputes the tile from x.
+// forward leaves behind, and recomputes the tile from x.
 #include "../../include/gdn_b200.h"
 
 #include <cooperative_groups.h>
@@ -33,19 +40,21 @@
 
 #include <cstdint>
 #include <cstring>
+#include <mutex>
 
 #include "host_util.h"
+#include "tc.cuh"
+#include "tmap.h"
 
 namespace gdn {
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCluster = 16;
 
 struct GscanParams {
+  CUtensorMap tm_x, tm_g, tm_d;  // (D, T, H, B) maps of x, g, d_o, for the tiles that TMA fetches
   const void* x;
   const void* g;
   const void* d_o;  // backward: gradient of o, or NULL (zero)
@@ -58,9 +67,10 @@ struct GscanParams {
   float* dh0;
   float* states;  // [B, NT, C] state before each tile, or NULL (forward only)
   long long xs[3], gs[3], os[3], dos[3], dxs[3], dgs[3];
-  int B, T, C, D;  // C = H * D channels
+  int B, T, C, H, D;  // C = H * D channels (H = 1, D = C where all tensors are flat)
   int NT, S;       // tiles of the sequence, CTAs per cluster
   int logits;      // g holds logits: a = sigmoid(g)
+  int* status;
 };
 
 // ---------------------------------------------------------------- vectors
@@ -79,6 +89,22 @@ struct Vec {
     __device__ U() {}
   };
   static __device__ __forceinline__ R load(const T* p) { return __ldcs(reinterpret_cast<const R*>(p)); }
+  // Asynchronous copy into this thread's shared-memory slot; 2-byte vectors
+  // (odd 16-bit tensors) are too small for one and are copied at once.
+  static __device__ __forceinline__ void fetch(R* slot, const T* p) {
+    if constexpr (sizeof(R) >= 4)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(uint32_t(__cvta_generic_to_shared(slot))), "l"(p),
+                   "n"(int(sizeof(R)))
+                   : "memory");
+    else
+      *slot = __ldcs(reinterpret_cast<const R*>(p));
+  }
+  static __device__ __forceinline__ R fill(float v) {
+    U u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) u.e[i] = T(v);
+    return u.r;
+  }
   static __device__ __forceinline__ void unpack(R r, float* f) {
     U u;
     u.r = r;
@@ -93,271 +119,471 @@ struct Vec {
   }
 };
 
-// Rows per warp: 8 for 16-bit x.  fp32 x takes 4, so that the backward's four
-// arrays of R x V values stay in registers.
-template <typename XT> __host__ __device__ constexpr int rows_per_warp() { return sizeof(XT) == 4 ? 4 : 8; }
+// A tile has 128 rows of 16-bit x or 64 of fp32 x, in the forward (whose tile
+// states the backward reads) and the backward alike.  The forward gives them
+// to few warps with many rows each: fewer maps to compose, and registers hold
+// one value per element.  The backward holds two, so twice the warps.
+// Measured for the forward (2 x 4096 tokens, 1 x 65536, 8 x 2048; 2048 channels): 4 warps of
+// 32 rows 25.3, 166, 37 us; 8 of 16 rows 24.4, 171, 44; 8 of 8 rows (64-row
+// tiles) 25.6, 212, 45.  Four channels per thread instead of two: 25.4, 203, 44.
+template <typename XT, bool BWD>
+struct Shape {
+  static constexpr int W = BWD ? 8 : 4;                                  // warps
+  static constexpr int TC = sizeof(XT) == 4 ? 64 : 128;                  // rows of a tile
+  static constexpr int R = TC / W;                                       // rows per warp
+  static constexpr int T = W * 32;                                       // threads
+};
+constexpr int kVec = 2;  // channels per thread where TMA fetches the tiles
 
-// a_t.  expf, not the raw exponential instruction: an error in a is multiplied
-// by the chain's memory length, and the final state is returned in fp32.
-__device__ __forceinline__ float decay(float g, bool logits) {
-  return logits ? __frcp_rn(1.f + expf(-g)) : expf(g);
+// Gates.  The hardware's base-2 exponential and reciprocal (2^-22 and 1 ulp) on
+// plain products: the argument's own rounding adds |g| ulp, but a gate with a
+// large |g| forgets at once, so the state's error stays a few ulp times its
+// magnitude; near 1, where errors add up over the chain's memory, it is none.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
 
+template <bool LOGITS>
+__device__ __forceinline__ float decay(float g) {
+  return LOGITS ? rcp(1.f + ex2(-kLog2e * g)) : ex2(kLog2e * g);
+}
 // The backward needs a and, for logits, 1 - a, each with its own relative
-// accuracy: s = min(a, 1 - a) = e / (1 + e), e = exp(-|g|), is kept with the
-// side it belongs to in the sign bit.
-__device__ __forceinline__ float pack_decay(float g, bool logits) {
-  if (!logits) return expf(g);
-  const float e = expf(-fabsf(g));
-  const float s = e * __frcp_rn(1.f + e);
-  return g < 0.f ? s : -s;
+// accuracy (1 - a is the gate's gradient, and small where the memory is long):
+// s = min(a, 1 - a) = e / (1 + e), e = exp(-|g|), with the sign bit set where s is 1 - a.
+template <bool LOGITS>
+__device__ __forceinline__ float pack_decay(float g) {
+  if (!LOGITS) return ex2(kLog2e * g);
+  const float e = ex2(-kLog2e * fabsf(g));
+  const float s = e * rcp(1.f + e);
+  return __uint_as_float(__float_as_uint(s) | (~__float_as_uint(g) & 0x80000000u));
 }
-__device__ __forceinline__ float decay_of(float p, bool logits) {
-  return logits && (__float_as_uint(p) >> 31) ? 1.f + p : p;
+template <bool LOGITS>
+__device__ __forceinline__ float decay_of(float p) {
+  return LOGITS && int(__float_as_uint(p)) < 0 ? 1.f + p : p;
 }
-__device__ __forceinline__ float slope_of(float p) { return (__float_as_uint(p) >> 31) ? -p : 1.f - p; }
+__device__ __forceinline__ float slope_of(float p) { return int(__float_as_uint(p)) < 0 ? -p : 1.f - p; }
 
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// Shared memory of one CTA, in bytes.  With bulk copies x and d_o have two
+// buffers: they are read a second time, when the rows are replayed, so that
+// registers hold the gates alone.
+template <typename XT, typename GT, typename OT, int V, bool BWD>
+struct Smem {
+  static constexpr bool kBulk = V > 1;
+  using Sh = Shape<XT, BWD>;
+  static constexpr int W = Sh::W, R = Sh::R, CB = 32 * V, N = Sh::TC * CB;  // elements of a tile
+  static constexpr int nb = kBulk ? 2 : 1;
+  static constexpr int x = 0;
+  static constexpr int g = x + nb * N * int(sizeof(XT));
+  static constexpr int d = g + N * int(sizeof(GT));                        // (backward)
+  static constexpr int map = d + (BWD ? nb * N * int(sizeof(OT)) : 0);     // [W][CB] float2
+  static constexpr int in = map + W * CB * 8;                         // [W][CB] float or float2
+  static constexpr int fx = in + W * CB * (BWD ? 8 : 4);              // [W][CB] float (backward)
+  static constexpr int bar = fx + (BWD ? W * CB * 4 : 0);             // mbarriers, the abort flag
+  static constexpr int agg = bar + 64;                                     // [2][S][CB] float2
+  static constexpr int bytes(int S) { return agg + (S > 1 ? 2 * S * CB * 8 : 0); }
+};
+enum { B_MAP = 0, B_DATA = 2, B_COUNT = 4 };  // two barriers each, used in turn
+
+// ---------------------------------------------------------------- exchange
+// A CTA's map of a stride goes to every CTA of its cluster by asynchronous
+// stores that count on the receiver's mbarrier.  Unlike a cluster barrier this
+// orders nothing else: no thread waits for its output stores to land, and only
+// the column owners wait for the maps.  Two buffers and barriers alternate: a
+// CTA sends the maps of stride i + 2 only after it has all those of i + 1,
+// whose senders had read stride i's.
+__device__ __forceinline__ uint32_t peer_addr(uint32_t local, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void push_map(uint32_t slot, uint32_t bar, int rank, float2 m) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(
+                   peer_addr(slot, rank)),
+               "l"((uint64_t(__float_as_uint(m.y)) << 32) | __float_as_uint(m.x)), "r"(peer_addr(bar, rank))
+               : "memory");
+}
+
+__device__ __forceinline__ float2 compose(float2 later, float2 m) {
+  return make_float2(later.x * m.x, fmaf(later.x, m.y, later.y));
+}
+
+// Where a CTA works: its chain's batch and columns, its place in the cluster.
 struct Place {
-  int b, ch0, rank;
-  bool live;
-  long long xo, go;  // element offsets of this thread's channels at t = 0
+  int b, h, d0, width, rank;
+  long long col0;  // first column among the B * C of the states
+};
+__device__ __forceinline__ Place place(const GscanParams& p, int CB) {
+  const int nd = (p.D + CB - 1) / CB;
+  const int chain = blockIdx.x / p.S;
+  Place q;
+  q.rank = blockIdx.x - chain * p.S;
+  const int hd = chain % (p.H * nd);
+  q.b = chain / (p.H * nd);
+  q.h = hd / nd;
+  q.d0 = (hd - q.h * nd) * CB;
+  q.width = p.D - q.d0 < CB ? p.D - q.d0 : CB;
+  q.col0 = (long long)q.h * p.D + q.d0;
+  return q;
+}
+__device__ __forceinline__ long long offset(const long long* st, const Place& q) {
+  return st[0] * q.b + st[2] * q.h + q.d0;
+}
+
+// One tensor's tiles on their way through shared memory.
+template <typename T, int V, int R>
+struct Tile {
+  static constexpr int CB = 32 * V;
+  static constexpr bool kBulk = V > 1;
+  const T* p;        // the CTA's columns at t = 0
+  long long stride;  // elements per row
+
+  // One channel per thread: this thread's rows, n of them there.
+  __device__ __forceinline__ void own(T* buf, long long t0, int n, bool live, T pad) const {
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      T* slot = buf + (w * R + r) * CB + lane;
+      if (r < n && live)
+        Vec<T, 1>::fetch(reinterpret_cast<typename Vec<T, 1>::R*>(slot), p + (t0 + w * R + r) * stride + lane);
+      else
+        *slot = pad;
+    }
+  }
+  static __device__ __forceinline__ const typename Vec<T, V>::R* at(const T* buf, int r) {
+    return reinterpret_cast<const typename Vec<T, V>::R*>(buf + ((threadIdx.x >> 5) * R + r) * CB) + (threadIdx.x & 31);
+  }
+  // Rows n.. of this thread's columns that no copy filled.
+  static __device__ __forceinline__ void pad(T* buf, int n, float v) {
+    for (int r = n; r < R; ++r)
+      *(reinterpret_cast<typename Vec<T, V>::R*>(buf + ((threadIdx.x >> 5) * R + r) * CB) + (threadIdx.x & 31)) =
+          Vec<T, V>::fill(v);
+  }
 };
 
-template <int V>
-__device__ __forceinline__ long long chan_off(const long long* st, int b, int ch, int D) {
-  const int h = ch / D;
-  return st[0] * b + st[2] * h + (ch - h * D);
+__device__ __forceinline__ void start(uint64_t* bars, volatile int* abort_flag, int S) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < B_COUNT; ++i) mbar_init(&bars[i], 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  // every barrier is ready before the first copy or map arrives
+  if (S > 1)
+    cg::this_cluster().sync();
+  else
+    __syncthreads();
+}
+
+// No CTA leaves while a map may still be on its way to it; a wait that ran out is reported.
+__device__ __forceinline__ void leave(int S, int* status, const volatile int* abort_flag) {
+  if (S > 1)
+    cg::this_cluster().sync();
+  else
+    __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && status) atomicOr(status, 1 << GDN_ERR_TIMEOUT);
+}
+
+// A tile's copies are waited for after an abort too: none may land in a CTA that has left.
+__device__ __forceinline__ void wait_data(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  volatile int own = 0;
+  if (!mbar_wait(bar, parity, &own)) *abort_flag = 1;
+}
+
+// Send this CTA's map of a column to the whole cluster, and wait for the others'.
+template <int CB>
+__device__ __forceinline__ void exchange(float2 m, float2* s_agg, uint64_t* bars, int k, int S, int rank,
+                                         volatile int* abort_flag) {
+  const int buf = k & 1;
+  uint64_t* bar = &bars[B_MAP + buf];
+  if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, uint32_t(S * CB * 8));
+  const uint32_t mine = smem_u32(s_agg + (buf * S + rank) * CB + threadIdx.x), b = smem_u32(bar);
+  for (int r = 0; r < S; ++r) push_map(mine, b, r, m);
+  if (!*abort_flag) mbar_wait(bar, (k >> 1) & 1, abort_flag);
 }
 
 // ---------------------------------------------------------------- forward
-template <typename XT, typename GT, typename OT, int V>
-__global__ void __launch_bounds__(kThreads, 2) gscan_fwd_kernel(const GscanParams p) {
-  constexpr int R = rows_per_warp<XT>();
-  constexpr int CB = 32 * V;
-  constexpr int TC = kWarps * R;
-  extern __shared__ float4 smem_raw[];
-  float2* s_map = reinterpret_cast<float2*>(smem_raw);       // [kWarps][CB] maps of this CTA's warps
-  float* s_in = reinterpret_cast<float*>(s_map + kWarps * CB);  // [kWarps][CB] state before each warp's rows
-  float2* s_agg = reinterpret_cast<float2*>(s_in + kWarps * CB);  // [2][S][CB] maps of the cluster's CTAs
+template <typename XT, typename GT, typename OT, int V, bool LOGITS>
+__global__ void __launch_bounds__(Shape<XT, false>::T, 4) gscan_fwd_kernel(const __grid_constant__ GscanParams p) {
+  using L = Smem<XT, GT, OT, V, false>;
+  using VX = Vec<XT, V>;
+  using VG = Vec<GT, V>;
+  constexpr int R = L::R, W = L::W, CB = L::CB, TC = W * R;
+  constexpr bool kBulk = L::kBulk;
+  extern __shared__ __align__(128) uint8_t sm[];
+  XT* s_x = reinterpret_cast<XT*>(sm + L::x);
+  GT* s_g = reinterpret_cast<GT*>(sm + L::g);
+  float2* s_map = reinterpret_cast<float2*>(sm + L::map);  // maps of this CTA's warps
+  float* s_in = reinterpret_cast<float*>(sm + L::in);      // state before each warp's rows
+  float2* s_agg = reinterpret_cast<float2*>(sm + L::agg);  // maps of the cluster's CTAs
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::bar);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::bar + 48);
 
-  cg::cluster_group cluster = cg::this_cluster();
-  const int S = p.S;
-  const int nblk = (p.C + CB - 1) / CB;
-  const int chain = blockIdx.x / S, rank = blockIdx.x - chain * S;
-  const int b = chain / nblk, cb = chain - b * nblk;
+  const Place q = place(p, CB);
+  const int S = p.S, rank = q.rank;
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  const int ch = cb * CB + lane * V;
-  const bool live = ch < p.C;
-  const XT* xp = static_cast<const XT*>(p.x) + (live ? chan_off<V>(p.xs, b, ch, p.D) : 0);
-  const GT* gp = static_cast<const GT*>(p.g) + (live ? chan_off<V>(p.gs, b, ch, p.D) : 0);
-  OT* op = static_cast<OT*>(p.o) + (live ? chan_off<V>(p.os, b, ch, p.D) : 0);
-  const bool logits = p.logits != 0;
-
-  // the running state, held by the thread that owns the column
-  const int col = cb * CB + tid;
-  const bool owner = tid < CB && col < p.C;
-  float H = (owner && p.h0) ? p.h0[(long long)b * p.C + col] : 0.f;
-
-  int buf = 0;
-  for (int tile0 = 0; tile0 < p.NT; tile0 += S, buf ^= 1) {
-    const int tile = tile0 + rank;
-    const long long t0 = (long long)tile * TC + w * R;
-    const int n = !live || t0 >= p.T ? 0 : (p.T - t0 < R ? int(p.T - t0) : R);
-    typename Vec<XT, V>::R xr[R];
-    typename Vec<GT, V>::R gr[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (r < n) {
-        xr[r] = Vec<XT, V>::load(xp + (t0 + r) * p.xs[1]);
-        gr[r] = Vec<GT, V>::load(gp + (t0 + r) * p.gs[1]);
+  const bool live = lane * V < q.width;
+  const Tile<XT, V, R> tx{static_cast<const XT*>(p.x) + offset(p.xs, q), p.xs[1]};
+  const Tile<GT, V, R> tg{static_cast<const GT*>(p.g) + offset(p.gs, q), p.gs[1]};
+  OT* op = static_cast<OT*>(p.o) + offset(p.os, q) + lane * V;
+  const float gpad = LOGITS ? INFINITY : 0.f;  // a = 1
+  auto rows_of = [&](int tile, int first, int most) {  // rows first .. first + most of a tile that exist
+    const long long t = (long long)tile * TC + first;
+    return t >= p.T ? 0 : (p.T - t < most ? int(p.T - t) : most);
+  };
+  auto fetch = [&](int tile, int k) {
+    const long long t0 = (long long)tile * TC;
+    if constexpr (kBulk) {
+      if (tid == 0) {
+        uint64_t* bar = &bars[B_DATA + (k & 1)];
+        mbar_arrive_expect_tx(bar, uint32_t(L::N) * uint32_t(sizeof(XT) + sizeof(GT)));
+        tma_load_4d(s_x + (k & 1) * L::N, &p.tm_x, bar, q.d0, int(t0), q.h, q.b);
+        tma_load_4d(s_g, &p.tm_g, bar, q.d0, int(t0), q.h, q.b);
       }
+    } else {
+      const int n = rows_of(tile, w * R, R);
+      tx.own(s_x, t0, n, live, XT(0.f));
+      tg.own(s_g, t0, n, live, GT(gpad));
+      cp_commit();
+    }
+  };
+
+  start(bars, abort_flag, S);
+  fetch(rank, 0);
+  // the running state, held by the thread that owns the column
+  const bool owner = tid < q.width;
+  const long long col = q.col0 + tid;
+  float H = (owner && p.h0) ? p.h0[(long long)q.b * p.C + col] : 0.f;
+
+  int k = 0;
+  for (int tile0 = 0; tile0 < p.NT; tile0 += S, ++k) {
+    const int tile = tile0 + rank;
+    const int n = rows_of(tile, w * R, R);
+    const XT* bx = s_x + (kBulk ? (k & 1) * L::N : 0);
+    if constexpr (kBulk) {
+      wait_data(&bars[B_DATA + (k & 1)], (k >> 1) & 1, abort_flag);
+      if (LOGITS && n < R) Tile<GT, V, R>::pad(s_g, n, gpad);  // TMA left 0 there: a = 1 only for log decays
+    } else {
+      cp_wait();
+    }
+    typename VX::R xr[kBulk ? 1 : R];
     float a[R][V], A[V], X[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.f, X[i] = 0.f;
-#pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (r < n) {
-        float xv[V], gv[V];
-        Vec<XT, V>::unpack(xr[r], xv);
-        Vec<GT, V>::unpack(gr[r], gv);
+      float xv[V], gv[V];
+      const typename VX::R xw = *Tile<XT, V, R>::at(bx, r);
+      if constexpr (!kBulk) xr[r] = xw;
+      VX::unpack(xw, xv);
+      VG::unpack(*Tile<GT, V, R>::at(s_g, r), gv);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          a[r][i] = decay(gv[i], logits);
-          X[i] = r == 0 ? xv[i] : fmaf(a[r][i], X[i], xv[i]);
-          A[i] *= a[r][i];
-        }
+      for (int i = 0; i < V; ++i) {
+        a[r][i] = decay<LOGITS>(gv[i]);
+        X[i] = r == 0 ? xv[i] : fmaf(a[r][i], X[i], xv[i]);
+        A[i] = r == 0 ? a[r][i] : A[i] * a[r][i];
       }
     }
+    if (!kBulk && tile0 + S < p.NT) fetch(tile + S, k + 1);
 #pragma unroll
     for (int i = 0; i < V; ++i) s_map[w * CB + lane * V + i] = make_float2(A[i], X[i]);
     __syncthreads();
-    if (S > 1) {
-      if (tid < CB) {
-        float2 m = s_map[tid];
-#pragma unroll
-        for (int j = 1; j < kWarps; ++j) {
-          const float2 n2 = s_map[j * CB + tid];
-          m = make_float2(n2.x * m.x, fmaf(n2.x, m.y, n2.y));
-        }
-        float2* mine = s_agg + (buf * S + rank) * CB + tid;
-        for (int r = 0; r < S; ++r) *cluster.map_shared_rank(mine, r) = m;
-      }
-      cluster.sync();
-    }
+    if (kBulk && tile0 + S < p.NT) fetch(tile + S, k + 1);
     if (tid < CB) {
-      const float2* agg = s_agg + buf * S * CB + tid;
-      for (int i = 0; i < rank; ++i) {
-        const float2 m = agg[i * CB];
-        H = fmaf(m.x, H, m.y);
-      }
-      if (p.states != nullptr && owner && tile < p.NT) p.states[((long long)b * p.NT + tile) * p.C + col] = H;
+      float2 wm[W];  // the column's map of each warp
 #pragma unroll
-      for (int j = 0; j < kWarps; ++j) {
+      for (int j = 0; j < W; ++j) wm[j] = s_map[j * CB + tid];
+      const float2* agg = s_agg + (k & 1) * S * CB + tid;
+      if (S > 1) {
+        float2 m = wm[0];
+#pragma unroll
+        for (int j = 1; j < W; ++j) m = compose(wm[j], m);
+        exchange<CB>(m, s_agg, bars, k, S, rank, abort_flag);
+        for (int i = 0; i < rank; ++i) H = fmaf(agg[i * CB].x, H, agg[i * CB].y);
+      }
+      if (p.states != nullptr && owner && tile < p.NT) p.states[((long long)q.b * p.NT + tile) * p.C + col] = H;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
         s_in[j * CB + tid] = H;
-        const float2 m = s_map[j * CB + tid];
-        H = fmaf(m.x, H, m.y);
+        H = fmaf(wm[j].x, H, wm[j].y);
       }
-      for (int i = rank + 1; i < S; ++i) {
-        const float2 m = agg[i * CB];
-        H = fmaf(m.x, H, m.y);
-      }
+      for (int i = rank + 1; i < S; ++i) H = fmaf(agg[i * CB].x, H, agg[i * CB].y);
     }
     __syncthreads();
     float h[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) h[i] = s_in[w * CB + lane * V + i];
+    OT* orow = op + ((long long)tile * TC + w * R) * p.os[1];
+    const int nl = live ? n : 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (r < n) {
-        float xv[V];
-        Vec<XT, V>::unpack(xr[r], xv);
+      float xv[V];
+      if constexpr (kBulk)
+        VX::unpack(*Tile<XT, V, R>::at(bx, r), xv);
+      else
+        VX::unpack(xr[r], xv);
 #pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = fmaf(a[r][i], h[i], xv[i]);
-        Vec<OT, V>::store(op + (t0 + r) * p.os[1], h);
-      }
+      for (int i = 0; i < V; ++i) h[i] = fmaf(a[r][i], h[i], xv[i]);
+      if (r < nl) Vec<OT, V>::store(orow, h);
+      orow += p.os[1];
     }
   }
-  if (rank == 0 && owner && p.ht) p.ht[(long long)b * p.C + col] = H;
+  leave(S, p.status, abort_flag);
+  if (rank == 0 && owner && p.ht) p.ht[(long long)q.b * p.C + col] = H;
 }
 
 // ---------------------------------------------------------------- backward
-template <typename XT, typename GT, typename OT, int V>
-__global__ void __launch_bounds__(kThreads, sizeof(XT) == 4 || sizeof(OT) == 4 ? 1 : 2)
-    gscan_bwd_kernel(const GscanParams p) {
-  constexpr int R = rows_per_warp<XT>();
-  constexpr int CB = 32 * V;
-  constexpr int TC = kWarps * R;
-  extern __shared__ float4 smem_raw[];
-  float2* s_map = reinterpret_cast<float2*>(smem_raw);       // [kWarps][CB] (A, M): mu maps, in reversed time
-  float2* s_in = s_map + kWarps * CB;                           // [kWarps][CB] (h before, mu behind) each warp's rows
-  float* s_x = reinterpret_cast<float*>(s_in + kWarps * CB);    // [kWarps][CB] X of the forward maps
-  float2* s_agg = reinterpret_cast<float2*>(s_x + kWarps * CB);  // [2][S][CB]
+template <typename XT, typename GT, typename OT, int V, bool LOGITS>
+__global__ void __launch_bounds__(Shape<XT, true>::T, 2) gscan_bwd_kernel(const __grid_constant__ GscanParams p) {
+  using L = Smem<XT, GT, OT, V, true>;
+  using VX = Vec<XT, V>;
+  using VG = Vec<GT, V>;
+  using VO = Vec<OT, V>;
+  constexpr int R = L::R, W = L::W, CB = L::CB, TC = W * R;
+  constexpr bool kBulk = L::kBulk;
+  extern __shared__ __align__(128) uint8_t sm[];
+  XT* s_x = reinterpret_cast<XT*>(sm + L::x);
+  GT* s_g = reinterpret_cast<GT*>(sm + L::g);
+  OT* s_d = reinterpret_cast<OT*>(sm + L::d);
+  float2* s_map = reinterpret_cast<float2*>(sm + L::map);  // (A, M) of each warp: maps of mu, in reversed time
+  float2* s_in = reinterpret_cast<float2*>(sm + L::in);    // (h before, mu behind) each warp's rows
+  float* s_fx = reinterpret_cast<float*>(sm + L::fx);      // X of each warp's forward map
+  float2* s_agg = reinterpret_cast<float2*>(sm + L::agg);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::bar);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::bar + 48);
 
-  cg::cluster_group cluster = cg::this_cluster();
-  const int S = p.S;
-  const int nblk = (p.C + CB - 1) / CB;
-  const int chain = blockIdx.x / S, rank = blockIdx.x - chain * S;
-  const int b = chain / nblk, cb = chain - b * nblk;
+  const Place q = place(p, CB);
+  const int S = p.S, rank = q.rank;
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  const int ch = cb * CB + lane * V;
-  const bool live = ch < p.C;
-  const XT* xp = static_cast<const XT*>(p.x) + (live ? chan_off<V>(p.xs, b, ch, p.D) : 0);
-  const GT* gp = static_cast<const GT*>(p.g) + (live ? chan_off<V>(p.gs, b, ch, p.D) : 0);
-  const OT* dop = static_cast<const OT*>(p.d_o) + (live ? chan_off<V>(p.dos, b, ch, p.D) : 0);
-  XT* dxp = static_cast<XT*>(p.dx) + (live ? chan_off<V>(p.dxs, b, ch, p.D) : 0);
-  GT* dgp = static_cast<GT*>(p.dg) + (live ? chan_off<V>(p.dgs, b, ch, p.D) : 0);
-  const bool logits = p.logits != 0, has_do = p.d_o != nullptr;
-
-  const int col = cb * CB + tid;
-  const bool owner = tid < CB && col < p.C;
-  float MU = (owner && p.dht) ? p.dht[(long long)b * p.C + col] : 0.f;
-
-  int buf = 0;
-  for (int tile0 = (p.NT - 1) / S * S; tile0 >= 0; tile0 -= S, buf ^= 1) {
-    const int tile = tile0 + rank;
-    const long long t0 = (long long)tile * TC + w * R;
-    const int n = !live || t0 >= p.T ? 0 : (p.T - t0 < R ? int(p.T - t0) : R);
-    typename Vec<XT, V>::R xr[R];
-    typename Vec<GT, V>::R gr[R];
-    typename Vec<OT, V>::R dr[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (r < n) {
-        xr[r] = Vec<XT, V>::load(xp + (t0 + r) * p.xs[1]);
-        gr[r] = Vec<GT, V>::load(gp + (t0 + r) * p.gs[1]);
-        if (has_do) dr[r] = Vec<OT, V>::load(dop + (t0 + r) * p.dos[1]);
+  const bool live = lane * V < q.width, has_do = p.d_o != nullptr;
+  const Tile<XT, V, R> tx{static_cast<const XT*>(p.x) + offset(p.xs, q), p.xs[1]};
+  const Tile<GT, V, R> tg{static_cast<const GT*>(p.g) + offset(p.gs, q), p.gs[1]};
+  const Tile<OT, V, R> td{has_do ? static_cast<const OT*>(p.d_o) + offset(p.dos, q) : nullptr, p.dos[1]};
+  XT* dxp = static_cast<XT*>(p.dx) + offset(p.dxs, q) + lane * V;
+  GT* dgp = static_cast<GT*>(p.dg) + offset(p.dgs, q) + lane * V;
+  const float gpad = LOGITS ? INFINITY : 0.f;  // a = 1
+  auto rows_of = [&](int tile, int first, int most) {
+    const long long t = (long long)tile * TC + first;
+    return t >= p.T ? 0 : (p.T - t < most ? int(p.T - t) : most);
+  };
+  auto fetch = [&](int tile, int k) {
+    const long long t0 = (long long)tile * TC;
+    if constexpr (kBulk) {
+      if (tid == 0) {
+        uint64_t* bar = &bars[B_DATA + (k & 1)];
+        mbar_arrive_expect_tx(bar, uint32_t(L::N) * uint32_t(sizeof(XT) + sizeof(GT) + (has_do ? sizeof(OT) : 0)));
+        tma_load_4d(s_x + (k & 1) * L::N, &p.tm_x, bar, q.d0, int(t0), q.h, q.b);
+        tma_load_4d(s_g, &p.tm_g, bar, q.d0, int(t0), q.h, q.b);
+        if (has_do) tma_load_4d(s_d + (k & 1) * L::N, &p.tm_d, bar, q.d0, int(t0), q.h, q.b);
       }
-    float hs = 0.f;  // state before this tile, for the column's owner
-    if (owner && tile < p.NT) hs = p.states[((long long)b * p.NT + tile) * p.C + col];
+    } else {
+      const int n = rows_of(tile, w * R, R);
+      tx.own(s_x, t0, n, live, XT(0.f));
+      tg.own(s_g, t0, n, live, GT(gpad));
+      td.own(s_d, t0, has_do ? n : 0, live, OT(0.f));
+      cp_commit();
+    }
+  };
+
+  start(bars, abort_flag, S);
+  const bool owner = tid < q.width;
+  const long long col = q.col0 + tid;
+  const float* states = p.states + (long long)q.b * p.NT * p.C + col;
+  int tile = (p.NT - 1) / S * S + rank;
+  fetch(tile, 0);
+  float hs = owner && tile < p.NT ? states[(long long)tile * p.C] : 0.f;  // state before the tile
+  float MU = (owner && p.dht) ? p.dht[(long long)q.b * p.C + col] : 0.f;
+
+  for (int k = 0; tile >= 0; tile -= S, ++k) {
+    const int n = rows_of(tile, w * R, R);
+    const XT* bx = s_x + (kBulk ? (k & 1) * L::N : 0);
+    const OT* bd = s_d + (kBulk ? (k & 1) * L::N : 0);
+    if constexpr (kBulk) {
+      wait_data(&bars[B_DATA + (k & 1)], (k >> 1) & 1, abort_flag);
+      if ((LOGITS && n < R) || !has_do) {
+        if (LOGITS) Tile<GT, V, R>::pad(s_g, n, gpad);  // TMA left 0 there: a = 1 only for log decays
+        if (!has_do) Tile<OT, V, R>::pad(const_cast<OT*>(bd), 0, 0.f);
+        fence_async_smem();  // later copies write there again
+      }
+    } else {
+      cp_wait();
+    }
+    typename VX::R xr[kBulk ? 1 : R];
+    typename VO::R dr[kBulk ? 1 : R];
     float pa[R][V], A[V], X[V], M[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.f, X[i] = M[i] = 0.f;
-#pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (r < n) {
-        float xv[V], gv[V];
-        Vec<XT, V>::unpack(xr[r], xv);
-        Vec<GT, V>::unpack(gr[r], gv);
+      float xv[V], gv[V];
+      const typename VX::R xw = *Tile<XT, V, R>::at(bx, r);
+      if constexpr (!kBulk) {
+        xr[r] = xw;
+        dr[r] = *Tile<OT, V, R>::at(bd, r);
+      }
+      VX::unpack(xw, xv);
+      VG::unpack(*Tile<GT, V, R>::at(s_g, r), gv);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          pa[r][i] = pack_decay(gv[i], logits);
-          const float a = decay_of(pa[r][i], logits);
-          X[i] = r == 0 ? xv[i] : fmaf(a, X[i], xv[i]);
-          A[i] *= a;
-        }
+      for (int i = 0; i < V; ++i) {
+        pa[r][i] = pack_decay<LOGITS>(gv[i]);
+        const float a = decay_of<LOGITS>(pa[r][i]);
+        X[i] = r == 0 ? xv[i] : fmaf(a, X[i], xv[i]);
+        A[i] = r == 0 ? a : A[i] * a;
       }
     }
-    if (has_do) {
+    if (!kBulk && tile >= S) fetch(tile - S, k + 1);
 #pragma unroll
-      for (int r = R - 1; r >= 0; --r) {
-        if (r < n) {
-          float dv[V];
-          Vec<OT, V>::unpack(dr[r], dv);
+    for (int r = R - 1; r >= 0; --r) {
+      float dv[V];
+      if constexpr (kBulk)
+        VO::unpack(*Tile<OT, V, R>::at(bd, r), dv);
+      else
+        VO::unpack(dr[r], dv);
 #pragma unroll
-          for (int i = 0; i < V; ++i) M[i] = decay_of(pa[r][i], logits) * (dv[i] + M[i]);
-        }
-      }
+      for (int i = 0; i < V; ++i) M[i] = decay_of<LOGITS>(pa[r][i]) * (r == R - 1 ? dv[i] : dv[i] + M[i]);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       s_map[w * CB + lane * V + i] = make_float2(A[i], M[i]);
-      s_x[w * CB + lane * V + i] = X[i];
+      s_fx[w * CB + lane * V + i] = X[i];
     }
     __syncthreads();
-    if (S > 1) {
-      if (tid < CB) {
-        float2 m = s_map[(kWarps - 1) * CB + tid];
-#pragma unroll
-        for (int j = kWarps - 2; j >= 0; --j) {
-          const float2 n2 = s_map[j * CB + tid];
-          m = make_float2(n2.x * m.x, fmaf(n2.x, m.y, n2.y));
-        }
-        float2* mine = s_agg + (buf * S + rank) * CB + tid;
-        for (int r = 0; r < S; ++r) *cluster.map_shared_rank(mine, r) = m;
-      }
-      cluster.sync();
-    }
+    if (kBulk && tile >= S) fetch(tile - S, k + 1);
     if (tid < CB) {
-      const float2* agg = s_agg + buf * S * CB + tid;
-      for (int i = S - 1; i > rank; --i) {
-        const float2 m = agg[i * CB];
-        MU = fmaf(m.x, MU, m.y);
+      float2 wm[W];  // the column's maps of mu, and X of its forward maps
+      float wx[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        wm[j] = s_map[j * CB + tid];
+        wx[j] = s_fx[j * CB + tid];
+      }
+      const float2* agg = s_agg + (k & 1) * S * CB + tid;
+      if (S > 1) {
+        float2 m = wm[W - 1];
+#pragma unroll
+        for (int j = W - 2; j >= 0; --j) m = compose(wm[j], m);
+        exchange<CB>(m, s_agg, bars, k, S, rank, abort_flag);
+        for (int i = S - 1; i > rank; --i) MU = fmaf(agg[i * CB].x, MU, agg[i * CB].y);
+      }
+      // MU behind each warp's rows takes the place of its map's M
+#pragma unroll
+      for (int j = W - 1; j >= 0; --j) {
+        const float mu = MU;
+        MU = fmaf(wm[j].x, MU, wm[j].y);
+        wm[j].y = mu;
       }
 #pragma unroll
-      for (int j = 0; j < kWarps; ++j) {
-        s_in[j * CB + tid].x = hs;
-        hs = fmaf(s_map[j * CB + tid].x, hs, s_x[j * CB + tid]);
+      for (int j = 0; j < W; ++j) {
+        s_in[j * CB + tid] = make_float2(hs, wm[j].y);
+        hs = fmaf(wm[j].x, hs, wx[j]);
       }
-#pragma unroll
-      for (int j = kWarps - 1; j >= 0; --j) {
-        s_in[j * CB + tid].y = MU;
-        const float2 m = s_map[j * CB + tid];
-        MU = fmaf(m.x, MU, m.y);
-      }
-      for (int i = rank - 1; i >= 0; --i) {
-        const float2 m = agg[i * CB];
-        MU = fmaf(m.x, MU, m.y);
-      }
+      for (int i = rank - 1; i >= 0; --i) MU = fmaf(agg[i * CB].x, MU, agg[i * CB].y);
+      hs = owner && tile >= S ? states[(long long)(tile - S) * p.C] : 0.f;
     }
     __syncthreads();
     float h[V], mu[V], hp[R][V];
@@ -369,39 +595,45 @@ __global__ void __launch_bounds__(kThreads, sizeof(XT) == 4 || sizeof(OT) == 4 ?
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (r < n) {
-        float xv[V];
-        Vec<XT, V>::unpack(xr[r], xv);
+      float xv[V];
+      if constexpr (kBulk)
+        VX::unpack(*Tile<XT, V, R>::at(bx, r), xv);
+      else
+        VX::unpack(xr[r], xv);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          hp[r][i] = h[i];
-          h[i] = fmaf(decay_of(pa[r][i], logits), h[i], xv[i]);
-        }
+      for (int i = 0; i < V; ++i) {
+        hp[r][i] = h[i];
+        h[i] = fmaf(decay_of<LOGITS>(pa[r][i]), h[i], xv[i]);
       }
     }
+    const int nl = live ? n : 0;
+    const long long t0 = (long long)tile * TC + w * R;
+    XT* dxr = dxp + (t0 + R - 1) * p.dxs[1];
+    GT* dgr = dgp + (t0 + R - 1) * p.dgs[1];
 #pragma unroll
     for (int r = R - 1; r >= 0; --r) {
-      if (r < n) {
-        float lam[V], dgv[V];
-        if (has_do) {
-          Vec<OT, V>::unpack(dr[r], lam);
-        } else {
+      float lam[V], dgv[V];
+      if constexpr (kBulk)
+        VO::unpack(*Tile<OT, V, R>::at(bd, r), lam);
+      else
+        VO::unpack(dr[r], lam);
 #pragma unroll
-          for (int i = 0; i < V; ++i) lam[i] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          lam[i] += mu[i];
-          mu[i] = decay_of(pa[r][i], logits) * lam[i];
-          dgv[i] = mu[i] * hp[r][i];
-          if (logits) dgv[i] *= slope_of(pa[r][i]);
-        }
-        Vec<XT, V>::store(dxp + (t0 + r) * p.dxs[1], lam);
-        Vec<GT, V>::store(dgp + (t0 + r) * p.dgs[1], dgv);
+      for (int i = 0; i < V; ++i) {
+        lam[i] += mu[i];
+        mu[i] = decay_of<LOGITS>(pa[r][i]) * lam[i];
+        dgv[i] = mu[i] * hp[r][i];
+        if (LOGITS) dgv[i] *= slope_of(pa[r][i]);
       }
+      if (r < nl) {
+        VX::store(dxr, lam);
+        VG::store(dgr, dgv);
+      }
+      dxr -= p.dxs[1];
+      dgr -= p.dgs[1];
     }
   }
-  if (rank == 0 && owner && p.dh0) p.dh0[(long long)b * p.C + col] = MU;
+  leave(S, p.status, abort_flag);
+  if (rank == 0 && owner && p.dh0) p.dh0[(long long)q.b * p.C + col] = MU;
 }
 
 // ---------------------------------------------------------------- few tokens
@@ -411,24 +643,24 @@ template <typename XT, typename GT, typename OT, int V>
 __global__ void __launch_bounds__(128) gscan_short_kernel(const GscanParams p) {
   const long long i0 = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * V;
   if (i0 >= (long long)p.B * p.C) return;
-  const int b = int(i0 / p.C), ch = int(i0 - (long long)b * p.C);
-  const XT* xp = static_cast<const XT*>(p.x) + chan_off<V>(p.xs, b, ch, p.D);
-  const GT* gp = static_cast<const GT*>(p.g) + chan_off<V>(p.gs, b, ch, p.D);
-  OT* op = static_cast<OT*>(p.o) + chan_off<V>(p.os, b, ch, p.D);
-  float h[V];
+  const int b = int(i0 / p.C), ch = int(i0 - (long long)b * p.C), h = ch / p.D, d = ch - h * p.D;
+  const XT* xp = static_cast<const XT*>(p.x) + p.xs[0] * b + p.xs[2] * h + d;
+  const GT* gp = static_cast<const GT*>(p.g) + p.gs[0] * b + p.gs[2] * h + d;
+  OT* op = static_cast<OT*>(p.o) + p.os[0] * b + p.os[2] * h + d;
+  float s[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) h[i] = 0.f;
-  if (p.h0) Vec<float, V>::unpack(Vec<float, V>::load(p.h0 + i0), h);
+  for (int i = 0; i < V; ++i) s[i] = 0.f;
+  if (p.h0) Vec<float, V>::unpack(Vec<float, V>::load(p.h0 + i0), s);
 #pragma unroll 4
   for (int t = 0; t < p.T; ++t) {
     float xv[V], gv[V];
     Vec<XT, V>::unpack(Vec<XT, V>::load(xp + t * p.xs[1]), xv);
     Vec<GT, V>::unpack(Vec<GT, V>::load(gp + t * p.gs[1]), gv);
 #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = fmaf(decay(gv[i], p.logits != 0), h[i], xv[i]);
-    Vec<OT, V>::store(op + t * p.os[1], h);
+    for (int i = 0; i < V; ++i) s[i] = fmaf(p.logits ? decay<true>(gv[i]) : decay<false>(gv[i]), s[i], xv[i]);
+    Vec<OT, V>::store(op + t * p.os[1], s);
   }
-  if (p.ht) Vec<float, V>::store(p.ht + i0, h);
+  if (p.ht) Vec<float, V>::store(p.ht + i0, s);
 }
 
 // ------------------------------------------------------------------ host side
@@ -436,54 +668,110 @@ constexpr int kShortRows = 16;
 
 enum class Pass { kFwd, kBwd };
 
-template <typename K>
-int launch_cluster(K kern, const GscanParams& p, int chains, size_t smem, cudaStream_t s, bool* configured) {
-  if (!*configured) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024) != cudaSuccess)
-      return cuda_failed();
-    *configured = true;
-  }
+// Per kernel and device: whether its attributes are set, and how many clusters
+// of each size the device holds at once.
+struct ClusterInfo {
+  bool ready;
+  int active[kMaxCluster + 1];
+};
+
+inline void cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* at, int clusters, int S, int threads, size_t smem,
+                           cudaStream_t s) {
+  memset(cfg, 0, sizeof(*cfg));
+  cfg->gridDim = dim3(unsigned(clusters) * unsigned(S));
+  cfg->blockDim = dim3(unsigned(threads));
+  cfg->dynamicSmemBytes = smem;
+  cfg->stream = s;
+  at->id = cudaLaunchAttributeClusterDimension;
+  at->val.clusterDim.x = unsigned(S);
+  at->val.clusterDim.y = at->val.clusterDim.z = 1;
+  cfg->attrs = at;
+  cfg->numAttrs = 1;
+}
+
+template <typename L, typename K>
+int launch_cluster(K kern, GscanParams p, int chains, cudaStream_t s, ClusterInfo* info) {
   cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(unsigned(chains) * unsigned(p.S));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
   cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = unsigned(p.S);
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  static std::mutex mu;
+  std::unique_lock<std::mutex> lock(mu);
+  if (!info->ready) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes(kMaxCluster)) != cudaSuccess)
+      return cuda_failed();
+    for (int S = 1; S <= kMaxCluster; ++S) {
+      cluster_config(&cfg, &at, 1, S, L::Sh::T, L::bytes(S), nullptr);
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+      }
+      info->active[S] = n;
+    }
+    info->ready = true;
+  }
+  lock.unlock();
+  // Cluster size: the fewest rounds of strides.  A size that leaves SMs empty
+  // or needs a second wave of clusters has more of them.
+  int best = 1;
+  long long best_cost = -1;
+  for (int S = 1; S <= kMaxCluster && S <= p.NT; ++S) {
+    if (info->active[S] < 1) continue;
+    const long long waves = (chains + info->active[S] - 1) / info->active[S];
+    const long long cost = waves * ((p.NT + S - 1) / S);
+    if (best_cost < 0 || cost < best_cost) best = S, best_cost = cost;
+  }
+  p.S = best;
+  cluster_config(&cfg, &at, chains, best, L::Sh::T, L::bytes(best), s);
   return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? GDN_OK : cuda_failed();
 }
 
-template <typename XT, typename GT, typename OT, int V>
+template <typename T> constexpr CUtensorMapDataType map_type();
+template <> constexpr CUtensorMapDataType map_type<float>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT32; }
+template <> constexpr CUtensorMapDataType map_type<__half>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
+template <> constexpr CUtensorMapDataType map_type<__nv_bfloat16>() { return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
+
+template <typename T>
+bool make_map(CUtensorMap* m, const GscanParams& p, const void* base, const long long* st, int columns, int rows) {
+  const uint64_t dims[4] = {uint64_t(p.D), uint64_t(p.T), uint64_t(p.H), uint64_t(p.B)};
+  // a dimension of one element may come with any stride: it is never taken
+  auto bytes = [&](long long s, int n) { return uint64_t(n > 1 ? s : p.D) * sizeof(T); };
+  const uint64_t strides[3] = {bytes(st[1], p.T), bytes(st[2], p.H), bytes(st[0], p.B)};
+  const uint32_t box[4] = {uint32_t(columns), uint32_t(rows), 1, 1};
+  return make_tmap(m, map_type<T>(), 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <typename XT, typename GT, typename OT, int V, bool LOGITS>
 int launch(GscanParams p, Pass pass, cudaStream_t s, int dev) {
-  constexpr int CB = 32 * V, TC = kWarps * rows_per_warp<XT>();
+  constexpr int CB = 32 * V, TC = Shape<XT, false>::TC;
+  p.NT = (p.T + TC - 1) / TC;
+  if (V > 1) {
+    if (!make_map<XT>(&p.tm_x, p, p.x, p.xs, CB, TC) || !make_map<GT>(&p.tm_g, p, p.g, p.gs, CB, TC)) return GDN_ERR_CUDA;
+    if (pass == Pass::kBwd && p.d_o && !make_map<OT>(&p.tm_d, p, p.d_o, p.dos, CB, TC)) return GDN_ERR_CUDA;
+  }
+  const long long chains = (long long)p.B * p.H * ((p.D + CB - 1) / CB);
+  if (chains * kMaxCluster > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED;
+  static ClusterInfo info[2][kMaxDevices] = {};
+  if (pass == Pass::kFwd)
+    return launch_cluster<Smem<XT, GT, OT, V, false>>(gscan_fwd_kernel<XT, GT, OT, V, LOGITS>, p, int(chains), s,
+                                                      &info[0][dev]);
+  return launch_cluster<Smem<XT, GT, OT, V, true>>(gscan_bwd_kernel<XT, GT, OT, V, LOGITS>, p, int(chains), s,
+                                                   &info[1][dev]);
+}
+
+template <typename XT, typename GT, typename OT, int V>
+int launch(const GscanParams& p, Pass pass, cudaStream_t s, int dev) {
   if (pass == Pass::kFwd && p.T <= kShortRows && p.states == nullptr) {
     const long long n = (long long)p.B * p.C / V;
     gscan_short_kernel<XT, GT, OT, V><<<unsigned((n + 127) / 128), 128, 0, s>>>(p);
     return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
   }
-  p.NT = (p.T + TC - 1) / TC;
-  const long long chains = (long long)p.B * ((p.C + CB - 1) / CB);
-  if (chains * kMaxCluster > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED;
-  int S = 1;
-  while (S < kMaxCluster && S < p.NT) S *= 2;
-  p.S = S;
-  static bool configured[2][kMaxDevices] = {};
-  if (pass == Pass::kFwd)
-    return launch_cluster(gscan_fwd_kernel<XT, GT, OT, V>, p, int(chains),
-                          size_t(CB) * (kWarps * 12 + (S > 1 ? 2 * S * 8 : 0)), s, &configured[0][dev]);
-  return launch_cluster(gscan_bwd_kernel<XT, GT, OT, V>, p, int(chains),
-                        size_t(CB) * (kWarps * 20 + (S > 1 ? 2 * S * 8 : 0)), s, &configured[1][dev]);
+  return p.logits ? launch<XT, GT, OT, V, true>(p, pass, s, dev) : launch<XT, GT, OT, V, false>(p, pass, s, dev);
 }
 
 template <typename XT, typename GT, typename OT>
 int launch_v(const GscanParams& p, Pass pass, int vec, cudaStream_t s, int dev) {
-  return vec == 4 ? launch<XT, GT, OT, 4>(p, pass, s, dev) : launch<XT, GT, OT, 1>(p, pass, s, dev);
+  return vec > 1 ? launch<XT, GT, OT, kVec>(p, pass, s, dev) : launch<XT, GT, OT, 1>(p, pass, s, dev);
 }
 
 template <typename XT>
@@ -492,11 +780,14 @@ int launch_x(const GscanParams& p, Pass pass, bool g32, bool o32, int vec, cudaS
   return o32 ? launch_v<XT, XT, float>(p, pass, vec, s, dev) : launch_v<XT, XT, XT>(p, pass, vec, s, dev);
 }
 
-// Whether `n`-element vectors of the tensor are aligned at every (b, t, h).
-bool vec_ok(const void* ptr, const int64_t* st, int es, int n) {
+// Whether every row of a tensor starts on, and is a multiple of, `align` bytes.
+bool row_ok(const void* ptr, const int64_t* st, const GscanParams& p, int es, int align) {
   if (ptr == nullptr) return true;
-  if (reinterpret_cast<uintptr_t>(ptr) % (size_t(es) * n)) return false;
-  return st[0] % n == 0 && st[1] % n == 0 && st[2] % n == 0;
+  if (reinterpret_cast<uintptr_t>(ptr) % size_t(align) || (long long)p.D * es % align) return false;
+  const int n[3] = {p.B, p.T, p.H};
+  for (int i = 0; st != nullptr && i < 3; ++i)
+    if (n[i] > 1 && (st[i] <= 0 || st[i] * es % align)) return false;
+  return true;
 }
 
 bool bad_stride(const int64_t* st) { return st[0] < 0 || st[1] < 0 || st[2] < 0; }
@@ -544,28 +835,36 @@ int run(const gdn_gated_scan_args* a, Pass pass, void* stream) {
   GscanParams p;
   memset(&p, 0, sizeof(p));
   p.x = a->x, p.g = a->g, p.h0 = a->h0, p.ht = a->ht, p.o = a->o, p.states = a->states;
-  p.B = a->B, p.T = a->T, p.C = a->H * a->D, p.D = a->D;
+  p.B = a->B, p.T = a->T, p.C = a->H * a->D, p.H = a->H, p.D = a->D;
   p.logits = (a->flags & GDN_FLAG_G_LOGSIGMOID) != 0;
+  p.status = a->status;
   copy3(p.xs, a->x_stride);
   copy3(p.gs, a->g_stride);
   copy3(p.os, a->o_stride);
   const int xe = dtype_size(a->x_dtype), ge = dtype_size(a->g_dtype), oe = dtype_size(a->o_dtype);
-  // Four channels per thread where every row of every tensor allows its
-  // vectors; one channel otherwise (odd head sizes, odd strides or bases).
-  bool v4 = a->D % 4 == 0 && vec_ok(a->x, a->x_stride, xe, 4) && vec_ok(a->g, a->g_stride, ge, 4);
+  const int64_t* in[3] = {a->x_stride, a->g_stride, pass == Pass::kBwd && a->d_o ? a->do_stride : a->x_stride};
+  const int64_t* out[2] = {pass == Pass::kFwd ? a->o_stride : a->dx_stride,
+                           pass == Pass::kFwd ? a->o_stride : a->dg_stride};
+  // Heads that lie one behind the other are one head.
+  bool flat = true;
+  for (auto st : {in[0], in[1], in[2], out[0], out[1]}) flat = flat && st[2] == a->D;
+  if (flat || a->H == 1) p.H = 1, p.D = p.C;
+  // TMA tiles and two channels per thread where every tensor's rows allow
+  // them; one channel otherwise (odd head sizes, odd strides or bases).
+  bool wide = row_ok(a->x, a->x_stride, p, xe, 16) && row_ok(a->g, a->g_stride, p, ge, 16);
   if (pass == Pass::kFwd) {
-    v4 = v4 && vec_ok(a->o, a->o_stride, oe, 4);
-    if (reinterpret_cast<uintptr_t>(a->h0) % 16 || reinterpret_cast<uintptr_t>(a->ht) % 16) v4 = false;
+    wide = wide && row_ok(a->o, a->o_stride, p, oe, kVec * oe) && row_ok(a->h0, nullptr, p, 4, 4 * kVec) &&
+         row_ok(a->ht, nullptr, p, 4, 4 * kVec);
   } else {
     p.d_o = a->d_o, p.dht = a->dht, p.dx = a->dx, p.dg = a->dg, p.dh0 = a->dh0;
     copy3(p.dos, a->do_stride);
     copy3(p.dxs, a->dx_stride);
     copy3(p.dgs, a->dg_stride);
-    v4 = v4 && vec_ok(a->d_o, a->do_stride, oe, 4) && vec_ok(a->dx, a->dx_stride, xe, 4) &&
-         vec_ok(a->dg, a->dg_stride, ge, 4);
+    wide = wide && row_ok(a->d_o, a->do_stride, p, oe, 16) && row_ok(a->dx, a->dx_stride, p, xe, kVec * xe) &&
+         row_ok(a->dg, a->dg_stride, p, ge, kVec * ge);
   }
   const bool g32 = a->g_dtype == GDN_DTYPE_F32, o32 = a->o_dtype == GDN_DTYPE_F32;
-  const int vec = v4 ? 4 : 1;
+  const int vec = wide ? kVec : 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->x_dtype == GDN_DTYPE_F32) return launch_v<float, float, float>(p, pass, vec, s, dev);
   if (a->x_dtype == GDN_DTYPE_F16) return launch_x<__half>(p, pass, g32, o32, vec, s, dev);
@@ -585,7 +884,6 @@ extern "C" int gdn_gated_scan_bwd_sm100(const gdn_gated_scan_args* args, void* s
 
 extern "C" uint64_t gdn_gated_scan_states_bytes(const gdn_gated_scan_args* a) {
   if (a == nullptr || a->B < 1 || a->T < 1 || a->H < 1 || a->D < 1) return 0;
-  const uint64_t rows = gdn::kWarps * (a->x_dtype == GDN_DTYPE_F32 ? gdn::rows_per_warp<float>()
-                                                                    : gdn::rows_per_warp<__half>());
+  const uint64_t rows = a->x_dtype == GDN_DTYPE_F32 ? gdn::Shape<float, false>::TC : gdn::Shape<__half, false>::TC;
   return uint64_t(a->B) * ((uint64_t(a->T) + rows - 1) / rows) * uint64_t(a->H) * uint64_t(a->D) * 4ull;
 }

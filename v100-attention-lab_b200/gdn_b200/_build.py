@@ -22,7 +22,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
     "-shared", "-Xcompiler", "-fPIC,-O2",
-    "-Xptxas", "-warn-spills",
+    "-Xptxas", "-warn-spills", "--threads=0",
 ]
 
 

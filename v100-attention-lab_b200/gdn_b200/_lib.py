@@ -108,6 +108,7 @@ class GatedScanArgs(ctypes.Structure):
         ("dg", ctypes.c_void_p),
         ("dg_stride", _i64x3),
         ("dh0", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
     ]
 
 
@@ -179,7 +180,7 @@ class StepArgs(ctypes.Structure):
 # The same structs as struct formats: one pack() fills a call's arguments
 # several times faster than setting ctypes fields, which counts for calls of
 # single tokens.  Native sizes and alignment; checked against the mirrors above.
-GATED_SCAN_ARGS = struct.Struct("@10iP3qP3qPP3qPPP3qPP3qP3qP")
+GATED_SCAN_ARGS = struct.Struct("@10iP3qP3qPP3qPPP3qPP3qP3qPP")
 WINDOW_ATTN_ARGS = struct.Struct("@10ifiP3qP3qP3qP3qPP")
 WINDOW_STEP_ARGS = struct.Struct("@9ifP2qP2qP2qP3qP3qP2qP")
 STEP_ARGS = struct.Struct("@8ifiP2qP2qP2qP2qP2qPP2q")

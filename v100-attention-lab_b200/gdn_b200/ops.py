@@ -79,6 +79,18 @@ def _status_word(device: torch.device) -> torch.Tensor:
     return w
 
 
+def _status_ptr(device: torch.device) -> int:
+    """Address of ``device``'s status word, or 0 if there is none yet and a graph is being captured.
+
+    A word made during a capture would live, and be cleared, with the graph."""
+    w = _status_words.get(device.index)
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        w = _status_word(device)
+    return w.data_ptr()
+
+
 def check_status(device=None) -> None:
     """Synchronise ``device`` and raise if any kernel launched there aborted.
 

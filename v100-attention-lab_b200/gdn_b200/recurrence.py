@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _check_device, _launch
+from .ops import _DTYPES, _check_device, _launch, _status_ptr
 
 __all__ = ["gated_scan", "gated_scan_step"]
 
@@ -68,7 +68,8 @@ def _pack(x, g, o_dtype, flags, h0=None, o=None, ht=None, states=None, d_o=None,
     return _lib.GATED_SCAN_ARGS.pack(
         _lib.ABI_VERSION, shape[0], shape[1] if len(shape) == 4 else 1, shape[-2], shape[-1],
         _DTYPES[x.dtype], _DTYPES[g.dtype], _DTYPES[o_dtype], flags, 0,
-        *_at(x), *_at(g), _ptr(h0), *_at(o), _ptr(ht), _ptr(states), *_at(d_o), _ptr(dht), *_at(dx), *_at(dg), _ptr(dh0))
+        *_at(x), *_at(g), _ptr(h0), *_at(o), _ptr(ht), _ptr(states), *_at(d_o), _ptr(dht), *_at(dx), *_at(dg), _ptr(dh0),
+        _status_ptr(x.device))
 
 
 def _forward(x, g, h0, flags, out_dtype, want_ht, want_states):
@@ -129,7 +130,7 @@ def gated_scan(x, g, initial_state=None, *, g_activation=None, output_dtype=None
 
     The state and all sums are fp32.  Differentiable (once) in x, g and
     initial_state; the backward recomputes the states in fp32 from x and g and
-    states kept every 32 (fp32 x) or 64 rows.  Results repeat bit for bit.
+    states kept every 64 (fp32 x) or 128 rows.  Results repeat bit for bit.
     Launches on the current stream of x's device without synchronising.
     """
     out_dtype = _check(x, g, initial_state, "initial_state", output_dtype, ("B", "T", "H", "D"))

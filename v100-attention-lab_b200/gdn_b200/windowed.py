@@ -14,8 +14,8 @@ import operator
 
 import torch
 
-from . import _lib, ops
-from .ops import _DTYPES, _check_device, _launch
+from . import _lib
+from .ops import _DTYPES, _check_device, _launch, _status_ptr
 
 __all__ = ["window_attention", "window_attention_step"]
 
@@ -101,17 +101,13 @@ def window_attention(q, k, v, window, sinks=0, *, scale=None, lengths=None):
     for name, t in tensors:
         _check_device(name, t, dev, "q")
     o = torch.empty((B, T, H, D), dtype=q.dtype, device=dev)
-    # The status word is made outside of graph captures: one made inside would
-    # live, and be cleared, with the graph.
-    status = 0
-    if dev.index in ops._status_words or not torch.cuda.is_current_stream_capturing():
-        status = ops._status_word(dev).data_ptr()
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), o.stride()
     args = _lib.WINDOW_ATTN_ARGS.pack(
         # beyond the keys neither window nor sinks change anything
         _lib.ABI_VERSION, B, T, S, H, HK, D, _DTYPES[q.dtype], min(window, S), min(sinks, S), scale, 0,
         q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2],
-        o.data_ptr(), so[0], so[1], so[2], 0 if lengths is None else lengths.data_ptr(), status)
+        o.data_ptr(), so[0], so[1], so[2], 0 if lengths is None else lengths.data_ptr(),
+        _status_ptr(dev))
     _launch(_lib.load().gdn_window_attn_sm100, "gdn_window_attn_sm100", args, dev)
     return o
 
