@@ -187,6 +187,17 @@ def test_single_gradients_and_broadcast_gates():
     assert not o5.requires_grad and torch.equal(o5, o)
 
 
+def test_second_derivative_is_refused():
+    import gdn_b200
+    x, g, h0, do, _ = make(1, 20, 1, 8, torch.float32, seed=4)
+    xl = x.requires_grad_()
+    (d0,) = torch.autograd.grad(gdn_b200.gated_scan(xl, g, h0)[0], xl, do)
+    (d1,) = torch.autograd.grad(gdn_b200.gated_scan(xl, g, h0)[0], xl, do.requires_grad_(), create_graph=True)
+    assert torch.equal(d0, d1)
+    with pytest.raises(RuntimeError, match="twice"):
+        d1.sum().backward()
+
+
 def test_strides_and_views():
     """Heads cut from a wider tensor, a base that no vector fits, time slices, expanded batches."""
     import gdn_b200
@@ -298,3 +309,31 @@ def test_offsets_past_32_bits():
     o, hT = gdn_b200.gated_scan(x, g)
     w, wT = gdn_b200.gated_scan(x.contiguous(), g)
     assert torch.equal(o, w) and torch.equal(hT, wT)
+
+
+def test_first_call_of_a_thread():
+    """A thread that has made no CUDA call yet has no current context; a first backward runs on such a thread."""
+    import subprocess
+    import sys
+    import textwrap
+    from conftest import ROOT
+    code = """
+    import sys, threading
+    sys.path.insert(0, "v100-attention-lab_b200")
+    import torch, gdn_b200
+    x = torch.nn.functional.normalize(torch.randn(1, 64, 2, 128, device="cuda"), dim=-1).bfloat16()
+    g = -torch.rand(1, 64, 2, 128, device="cuda")
+    b = torch.rand(1, 64, 2, device="cuda")
+    want = gdn_b200.gated_scan(x, g)[0], gdn_b200.window_attention(x, x, x, 9), gdn_b200.gdn_chunk_fwd(x, x, x, b, -b)[0]
+    xl = x.clone().requires_grad_()
+    torch.autograd.grad(gdn_b200.gated_scan(xl, g)[0].sum(), xl)
+    for i, f in enumerate((lambda: gdn_b200.gated_scan(x, g)[0], lambda: gdn_b200.window_attention(x, x, x, 9),
+                           lambda: gdn_b200.gdn_chunk_fwd(x, x, x, b, -b)[0])):
+        got = []
+        t = threading.Thread(target=lambda: got.append(f()))
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[i]), i
+    """
+    subprocess.run([sys.executable, "-c", textwrap.dedent(code)], check=True, cwd=ROOT, timeout=300)

@@ -40,9 +40,16 @@ inline bool make_tmap(CUtensorMap* map, CUtensorMapDataType dt, uint32_t rank, c
     es[i] = 1;
     if (i + 1 < rank) gs[i] = strides_bytes[i];
   }
-  CUresult r = fn(map, dt, rank, const_cast<void*>(base), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  auto encode = [&] {
+    return fn(map, dt, rank, const_cast<void*>(base), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (encode()) return true;
+  // A host thread that has made no runtime call yet (a backward's thread, a
+  // worker of the caller) has no current context, and the driver call fails:
+  // make the device's context current and try again.
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode();
 }
 
 }  // namespace gdn

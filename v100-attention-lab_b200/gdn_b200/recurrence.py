@@ -96,22 +96,31 @@ class _GatedScan(torch.autograd.Function):
         return o, ht
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, dht):
-        if d_o is None and dht is None:
-            return None, None, None, None, None, None
-        x, g, states = ctx.saved_tensors
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dg = torch.empty(g.shape, dtype=g.dtype, device=x.device)
-        need_x, need_g, need_h0 = ctx.needs_input_grad[:3]
-        dh0 = torch.empty((x.shape[0],) + x.shape[2:], dtype=torch.float32, device=x.device) if need_h0 else None
-        if d_o is not None and d_o.stride(-1) != 1:  # e.g. the expanded gradient of a sum
-            d_o = d_o.contiguous()
-        if dht is not None:
-            dht = dht.contiguous()
-        _launch(_lib.load().gdn_gated_scan_bwd_sm100, "gdn_gated_scan_bwd_sm100",
-                _pack(x, g, ctx.out_dtype, ctx.flags, states=states, d_o=d_o, dht=dht, dx=dx, dg=dg, dh0=dh0), x.device)
-        return dx if need_x else None, dg if need_g else None, dh0, None, None, None
+        # The wrapper that refuses a second derivative costs 20 us of host time;
+        # without create_graph nothing is recorded, and none can be asked for.
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, d_o, dht)
+
+
+def _backward(ctx, d_o, dht):
+    if d_o is None and dht is None:
+        return None, None, None, None, None, None
+    x, g, states = ctx.saved_tensors
+    dev = x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dg = torch.empty(x.shape, dtype=g.dtype, device=dev)
+    need_x, need_g, need_h0 = ctx.needs_input_grad[:3]
+    dh0 = torch.empty((x.shape[0],) + x.shape[2:], dtype=torch.float32, device=dev) if need_h0 else None
+    if d_o is not None and d_o.stride(-1) != 1:  # e.g. the expanded gradient of a sum
+        d_o = d_o.contiguous()
+    if dht is not None:
+        dht = dht.contiguous()
+    _launch(_lib.load().gdn_gated_scan_bwd_sm100, "gdn_gated_scan_bwd_sm100",
+            _pack(x, g, ctx.out_dtype, ctx.flags, states=states, d_o=d_o, dht=dht, dx=dx, dg=dg, dh0=dh0), dev)
+    return dx if need_x else None, dg if need_g else None, dh0, None, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def gated_scan(x, g, initial_state=None, *, g_activation=None, output_dtype=None, output_final_state=True):
