@@ -244,7 +244,6 @@ __device__ __forceinline__ long long offset(const long long* st, const Place& q)
 template <typename T, int V, int R>
 struct Tile {
   static constexpr int CB = 32 * V;
-  static constexpr bool kBulk = V > 1;
   const T* p;        // the CTA's columns at t = 0
   long long stride;  // elements per row
 

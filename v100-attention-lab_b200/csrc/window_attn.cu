@@ -11,20 +11,23 @@
 // visible key tiles.  Tensor cores bound it at 4 D operations per visible pair;
 // the exponentials (16 per clock and SM) take as long as the products do.
 //
-// Split.  A CTA owns two tiles of 128 query rows that share their keys: two
+// Split.  A work item is two tiles of 128 query rows that share their keys: two
 // heads of one key head where heads share keys in even groups, else two
 // neighbouring tiles of one head.  So every K/V tile fetched feeds two
 // products, and while one tile's softmax runs the tensor core works on the
-// other's.  Warps: 2 x 4 softmax (one thread per query row), one that
-// fetches K/V tiles by TMA, one that issues the MMAs.  TMEM holds both score
-// tiles and both outputs; the probabilities overwrite their scores' columns
-// and are the second product's TMEM operand, so they never touch shared memory.
+// other's.  One CTA per SM takes item after item; its loads and first scores
+// of the next item run under the last one's epilogue.  Warps: 2 x 4 softmax
+// (one thread per query row), one that fetches K/V tiles by TMA, one that
+// issues the MMAs.  TMEM holds both score tiles and both outputs; the
+// probabilities overwrite their scores' columns and are the second product's
+// TMEM operand, so they never touch shared memory.
 //
 // Masks.  Only tiles that some mask cuts are masked element by element.  In
-// those a key hidden from a row has probability 0, and 0 times a non-finite
-// value would still poison the row; so the values of a cut tile are looked
-// over, and if one is not finite its product is summed on the CUDA cores over
-// visible keys alone.
+// those a key hidden from a row has probability 0, and 0 times a value that is
+// not finite would still poison the row.  Such an output cannot be missed: it is
+// not finite itself.  Items with one are done again in a careful pass, which
+// looks the values of cut tiles over and sums those that hold a non-finite one
+// on the CUDA cores, over visible keys alone.
 #include "../../include/gdn_b200.h"
 #include "host_util.h"
 #include "tc.cuh"
@@ -44,6 +47,7 @@ constexpr int kTmaWarp = 8, kMmaWarp = 9;
 // Three warpgroups, so that registers can be moved between them: 168 each at
 // launch, then 2 x 216 for the softmax warps and 72 for the others (504 in all).
 constexpr int kThreads = 384;
+constexpr int kMaxItems = 8192;     // of one CTA
 constexpr uint32_t kTmCols = 512;
 constexpr uint32_t kTmS = 0, kTmO = 256;  // + 128 x tile
 
@@ -55,7 +59,8 @@ struct Params {
   long long so_b, so_t, so_h;
   int T, S, HK, G;
   int window, sinks;
-  int pair_heads;    // the CTA's two tiles are two heads (else two row tiles of one head)
+  int nx, ny, items;  // row tiles (or pairs) and heads (or pairs) of an item grid, items in all
+  int pair_heads;    // an item's two tiles are two heads (else two row tiles of one head)
   float scale_log2;  // scale * log2(e)
 };
 
@@ -66,14 +71,17 @@ struct Lay {
   static constexpr uint32_t stages = D == 128 ? 4 : 6;
   static constexpr uint32_t q = 0;                        // two query tiles
   static constexpr uint32_t kv = 2 * tile;                // ring of K and V tiles
-  static constexpr uint32_t bars = kv + stages * tile;
-  static constexpr uint32_t misc = bars + 8 * (2 * stages + 8);
-  static constexpr uint32_t bytes = misc + 64;
+  static constexpr uint32_t out = kv + stages * tile;      // [8 warps][32 rows][64 columns] of outputs
+  static constexpr uint32_t bars = out + 32768;
+  static constexpr uint32_t misc = bars + 8 * (2 * stages + 16);
+  static constexpr uint32_t redo = misc + 64;             // one bit per item of this CTA
+  static constexpr uint32_t bytes = redo + kMaxItems / 8;
   static constexpr uint32_t alloc = bytes + 1024;
 };
 
-// barriers behind the ring's full[stages], empty[stages]
-enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 6, B_COUNT = 8 };
+// Barriers behind the ring's full[stages], empty[stages]; two each, one per tile.
+// B_P: the first and, two on, the second half of the probabilities.
+enum { B_Q = 0, B_QE = 2, B_S = 4, B_P = 6, B_O = 10, B_OE = 12, B_COUNT = 14 };
 
 __device__ __forceinline__ void mma_f16_ts_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
                                                 uint32_t accumulate) {
@@ -97,7 +105,58 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), 
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 64 columns of this thread's TMEM lane, with the wait in the same statement.
+__device__ __forceinline__ void tmem_ld64w(uint32_t taddr, float* v) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+        "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
+        "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Two fp32 operations in one instruction.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 f2_get(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
 
 template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -112,51 +171,63 @@ template <> struct Pair<__nv_bfloat16> {
   using V = __nv_bfloat162;
 };
 
-// The CTA's key tiles, in order: those of the sinks, then those of the window.
-struct Tiles {
-  int n_sink, w0, count;
-  int p0[2];       // position of each query tile's first row
-  int p1[2];       // and of its last one that exists (p0 - 1: no rows)
+// One of a work item's two query tiles: which rows it has and which keys they see.
+struct Rows {
+  int p0, p1;  // positions of its first row and of its last one that exists (p1 < p0: no rows)
   int len, window, sinks;
 
-  __device__ __forceinline__ int key0(int u) const { return (u < n_sink ? u : w0 + (u - n_sink)) * kTile; }
-  // whether some row of query tile x sees a key of the tile at k0
-  __device__ __forceinline__ bool sees(int x, int k0) const {
-    if (p1[x] < p0[x] || p0[x] >= len || k0 >= len || k0 > p1[x]) return false;
-    return k0 < sinks || k0 + kTile > p0[x] - window + 1;
+  // whether it has a row that sees anything (then its first row sees itself)
+  __device__ __forceinline__ bool used() const { return p1 >= p0 && p0 < len; }
+  // whether some row sees a key of the tile at k0
+  __device__ __forceinline__ bool sees(int k0) const {
+    return used() && k0 < len && k0 <= p1 && (k0 < sinks || k0 + kTile > p0 - window + 1);
   }
-  // whether every row of query tile x sees every key of the tile at k0
-  __device__ __forceinline__ bool whole(int x, int k0) const {
+  // whether every row sees every key of the tile at k0
+  __device__ __forceinline__ bool whole(int k0) const {
     const int k1 = k0 + kTile - 1;
-    return k1 <= p0[x] && k1 < len && (k1 < sinks || p1[x] - k0 < window);
+    return k1 <= p0 && k1 < len && (k1 < sinks || p1 - k0 < window);
   }
 };
 
-__device__ __forceinline__ Tiles make_tiles(const Params& P, int len) {
-  Tiles t;
-  t.len = len;
-  t.window = P.window;
-  t.sinks = P.sinks;
-  const int row0 = blockIdx.x * (P.pair_heads ? kTile : 2 * kTile);
-  for (int x = 0; x < 2; ++x) {
-    const int r = row0 + (P.pair_heads ? 0 : x * kTile);
-    t.p0[x] = P.S - P.T + r;
-    const int last = r + kTile < P.T ? r + kTile : P.T;
-    t.p1[x] = P.S - P.T + last - 1;
+// A work item and its key tiles, in order: those of the sinks, then those of the window.
+// (All scalars: an array indexed by the tile would live in local memory, and
+// with this much shared memory taken, that means L2.)
+struct Item {
+  int b, hy, hk, row0;  // hy: the (first) query head
+  int len, n_sink, w0, count;
+
+  __device__ __forceinline__ int key0(int u) const { return (u < n_sink ? u : w0 + (u - n_sink)) * kTile; }
+  __device__ __forceinline__ int row(const Params& P, int x) const { return row0 + (P.pair_heads ? 0 : x * kTile); }
+  __device__ __forceinline__ int head(const Params& P, int x) const { return hy + (P.pair_heads ? x : 0); }
+  __device__ __forceinline__ Rows rows(const Params& P, int x) const {
+    const int r = row(P, x);
+    return Rows{P.S - P.T + r, P.S - P.T + (r + kTile < P.T ? r + kTile : P.T) - 1, len, P.window, P.sinks};
   }
-  int end = t.p1[1] > t.p1[0] ? t.p1[1] : t.p1[0];
-  if (end > len - 1) end = len - 1;
-  if (t.p0[0] >= len || end < 0) {
-    t.n_sink = t.w0 = t.count = 0;
-    return t;
+};
+
+__device__ __forceinline__ Item make_item(const Params& P, int i) {
+  Item it;
+  const int y = i / P.nx;
+  it.row0 = (i - y * P.nx) * (P.pair_heads ? kTile : 2 * kTile);
+  it.b = y / P.ny;
+  it.hy = (y - it.b * P.ny) * (P.pair_heads ? 2 : 1);
+  it.hk = it.hy / P.G;
+  it.len = P.S;
+  if (P.lengths) {
+    it.len = P.lengths[it.b];
+    it.len = it.len < 0 ? 0 : (it.len > P.S ? P.S : it.len);
   }
-  const int w1 = end / kTile;
-  const int lo = t.p0[0] - P.window + 1;
-  t.n_sink = P.sinks > 0 ? (P.sinks - 1) / kTile + 1 : 0;
-  t.w0 = lo > 0 ? lo / kTile : 0;
-  if (t.n_sink >= t.w0) t.n_sink = t.w0;  // the sinks' tiles run into the window's
-  t.count = t.n_sink + (w1 - t.w0 + 1);
-  return t;
+  const Rows r0 = it.rows(P, 0), r1 = it.rows(P, 1);
+  int end = r1.p1 > r0.p1 ? r1.p1 : r0.p1;
+  if (end > it.len - 1) end = it.len - 1;
+  it.n_sink = it.w0 = it.count = 0;
+  if (r0.p0 >= it.len) return it;
+  const int lo = r0.p0 - P.window + 1;
+  it.n_sink = P.sinks > 0 ? (P.sinks - 1) / kTile + 1 : 0;
+  it.w0 = lo > 0 ? lo / kTile : 0;
+  if (it.n_sink >= it.w0) it.n_sink = it.w0;  // the sinks' tiles run into the window's
+  it.count = it.n_sink + (end / kTile - it.w0 + 1);
+  return it;
 }
 
 // One column of this thread's TMEM lane (warp-collective).
@@ -213,6 +284,38 @@ __device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uin
   }
 }
 
+// Masked scores of one tile: this row's visible keys are those up to hi, from lo on or below sk.
+__device__ __forceinline__ void mask_row(float* s, int hi, int lo, int sk) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    // bits of the 32 columns from 32 w on
+    auto below = [&](int n) {  // columns < n
+      n -= 32 * w;
+      return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
+    };
+    const uint32_t see = below(hi + 1) & (~below(lo) | below(sk));
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+      if (!(see & (1u << c))) s[32 * w + c] = -INFINITY;
+  }
+}
+
+// Whether a value of this thread's key row of the tile is not finite (times 0 it is NaN).
+template <typename T, int D>
+__device__ __noinline__ bool row_not_finite(const uint8_t* vt, int r) {
+  using V2 = typename Pair<T>::V;
+  V2 acc = Pair<T>::zero();
+  for (int c = 0; c < D / 8; ++c) {
+    const uint4 w = *reinterpret_cast<const uint4*>(vt + (c >> 3) * 16384 + sw128_off(r, c & 7));
+    acc = __hfma2(*reinterpret_cast<const V2*>(&w.x), Pair<T>::zero(), acc);
+    acc = __hfma2(*reinterpret_cast<const V2*>(&w.y), Pair<T>::zero(), acc);
+    acc = __hfma2(*reinterpret_cast<const V2*>(&w.z), Pair<T>::zero(), acc);
+    acc = __hfma2(*reinterpret_cast<const V2*>(&w.w), Pair<T>::zero(), acc);
+  }
+  const float z = __low2float(acc) + __high2float(acc);
+  return z != z;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_constant__ Params P) {
   using L = Lay<D>;
@@ -224,19 +327,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   uint32_t* tmem_base_p = reinterpret_cast<uint32_t*>(sm + L::misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::misc + 4);
   volatile int* skip_pv = reinterpret_cast<volatile int*>(sm + L::misc + 8);  // [2]: the product is already in O
+  volatile int* any_redo = reinterpret_cast<volatile int*>(sm + L::misc + 16);
+  uint32_t* redo = reinterpret_cast<uint32_t*>(sm + L::redo);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t sb = smem_u32(sm);
-
-  const int b = blockIdx.z;
-  const int hy = P.pair_heads ? 2 * blockIdx.y : blockIdx.y;
-  const int hk = hy / P.G;
-  const int row0 = blockIdx.x * (P.pair_heads ? kTile : 2 * kTile);
-  int len = P.S;
-  if (P.lengths) {
-    len = P.lengths[b];
-    len = len < 0 ? 0 : (len > P.S ? P.S : len);
-  }
-  const Tiles tl = make_tiles(P, len);
 
   if (tid == 0) {
     for (uint32_t i = 0; i < L::stages; ++i) {
@@ -245,14 +339,19 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&bars[B_Q + x], 1);
+      mbar_init(&bars[B_QE + x], 1);
       mbar_init(&bars[B_S + x], 1);
       mbar_init(&bars[B_P + x], 4);
+      mbar_init(&bars[B_P + 2 + x], 4);
       mbar_init(&bars[B_O + x], 1);
+      mbar_init(&bars[B_OE + x], 4);
     }
     *abort_flag = 0;
+    *any_redo = 0;
     skip_pv[0] = skip_pv[1] = 0;
     fence_mbar_init();
   }
+  for (int i = tid; i < kMaxItems / 32; i += kThreads) redo[i] = 0;
   if (warp == kMmaWarp) {
     tmem_alloc(tmem_base_p, kTmCols);
     tmem_relinquish();
@@ -261,96 +360,130 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = *tmem_base_p;
 
+  // A second, careful pass follows if the first one noted any item; all warps meet in between.
+  auto again = [&](bool careful) {
+    named_bar(3, kThreads);
+    return !careful && *any_redo && !*abort_flag;
+  };
+  // Counts over all items and passes, for the barriers' phases:
+  uint32_t nkv = 0;           // ring slots used
+  uint32_t nq0 = 0, nq1 = 0;  // items that used query tile 0, 1 (softmax: the first for its own)
+  uint32_t ns0 = 0, ns1 = 0;  // key tiles of query tile 0, 1 (the same)
+  bool ok = true, careful = false;
+
   if (warp >= 8) {
     regs_less<72>();
-  if (warp == kTmaWarp) {
-    // ------------------------------------------------ producer: Q tiles, then K0 V0 K1 V1 ...
-    int loads = 0;
-    bool ok = true;
-    if (tl.count > 0) {
-      if (lane == 0) {
-        for (int x = 0; x < 2; ++x) {
-          if (tl.p1[x] < tl.p0[x]) continue;
-          mbar_arrive_expect_tx(&bars[B_Q + x], L::tile);
-          for (uint32_t c = 0; c < L::boxes; ++c)
-            tma_load_4d(sm + L::q + x * L::tile + c * 16384, &P.tm_q, &bars[B_Q + x], c * 64,
-                        row0 + (P.pair_heads ? 0 : x * kTile), hy + (P.pair_heads ? x : 0), b);
-        }
-      }
-      for (int u = 0; u < tl.count && ok; ++u) {
-        const int k0 = tl.key0(u);
-        for (int kv = 0; kv < 2; ++kv, ++loads) {
-          const int s = loads % L::stages;
-          if (loads >= int(L::stages) && !mbar_wait_warp(&empty[s], (loads / L::stages - 1) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&full[s], L::tile);
-            for (uint32_t c = 0; c < L::boxes; ++c)
-              tma_load_4d(sm + L::kv + s * L::tile + c * 16384, kv ? &P.tm_v : &P.tm_k, &full[s], c * 64, k0, hk, b);
-          }
-          __syncwarp();
-        }
-      }
-      // On an abort the loads still in flight land before the CTA leaves.
-      volatile int never = 0;
-      for (int x = 0; x < 2; ++x)
-        if (*abort_flag && tl.p1[x] >= tl.p0[x]) mbar_wait(&bars[B_Q + x], 0, &never);
-      for (int i = loads > int(L::stages) ? loads - int(L::stages) : 0; i < loads && *abort_flag; ++i)
-        mbar_wait(&full[i % L::stages], (i / L::stages) & 1, &never);
-    }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------ MMA issue (the whole warp; elect.sync inside)
-    constexpr uint32_t kBf16 = Cvt<T>::kIsBf16;
-    constexpr uint32_t id_s = idesc_f16(128, 128, kBf16, 0, 0), id_o = idesc_f16(128, D, kBf16, 0, 1);
-    bool ok = true;
-    uint32_t np[2] = {0, 0}, acc[2] = {0, 0};
-    bool got_q[2] = {false, false};
-    auto score = [&](int x, int u) {
-      const uint32_t q = sb + L::q + x * L::tile, k = sb + L::kv + ((2 * u) % L::stages) * L::tile;
+    do {
+      if (warp == kTmaWarp) {
+        // -------------------------------------------- producer: Q tiles, then K0 V0 K1 V1 ...
+        for (int j = 0, i = blockIdx.x; i < P.items && ok; ++j, i += gridDim.x) {
+          if (careful && !(redo[j >> 5] >> (j & 31) & 1)) continue;
+          const Item it = make_item(P, i);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        mma_f16_ss_warp(tmem + kTmS + x * 128, sdesc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024, kSw128),
-                        sdesc(k + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024, kSw128), id_s, kk > 0);
-      mma_commit_warp(&bars[B_S + x]);
-    };
-    auto wait_kv = [&](int i) { return mbar_wait_warp(&full[i % L::stages], (i / L::stages) & 1, abort_flag); };
-    for (int u = -1; u < tl.count && ok; ++u) {
-      for (int x = 0; x < 2 && ok; ++x) {
-        if (u >= 0 && tl.sees(x, tl.key0(u))) {
-          ok = wait_kv(2 * u + 1) && mbar_wait_warp(&bars[B_P + x], np[x] & 1, abort_flag);
-          if (!ok) break;
-          ++np[x];
-          tc_fence_after();
-          if (!skip_pv[x]) {
-            const uint32_t v = sb + L::kv + ((2 * u + 1) % L::stages) * L::tile;
-#pragma unroll
-            for (int kk = 0; kk < kTile / 16; ++kk)
-              mma_f16_ts_warp(tmem + kTmO + x * 128, tmem + kTmS + x * 128 + kk * 8,
-                              sdesc(v + kk * 2048, 16384, 1024, kSw128), id_o, acc[x] | (kk > 0));
+          for (int x = 0; x < 2; ++x) {
+            uint32_t& nq = x ? nq1 : nq0;
+            if (!ok || !it.rows(P, x).used()) continue;
+            if (nq > 0) ok = mbar_wait_warp(&bars[B_QE + x], (nq - 1) & 1, abort_flag);
+            if (!ok) continue;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&bars[B_Q + x], L::tile);
+              for (uint32_t c = 0; c < L::boxes; ++c)
+                tma_load_4d(sm + L::q + x * L::tile + c * 16384, &P.tm_q, &bars[B_Q + x], c * 64, it.row(P, x),
+                            it.head(P, x), it.b);
+            }
+            __syncwarp();
+            ++nq;
           }
-          acc[x] = 1;
+          for (int n = 0; n < 2 * it.count && ok; ++n) {
+            const uint32_t s = nkv % L::stages;
+            if (nkv >= L::stages) ok = mbar_wait_warp(&empty[s], (nkv / L::stages - 1) & 1, abort_flag);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&full[s], L::tile);
+              for (uint32_t c = 0; c < L::boxes; ++c)
+                tma_load_4d(sm + L::kv + s * L::tile + c * 16384, (n & 1) ? &P.tm_v : &P.tm_k, &full[s], c * 64,
+                            it.key0(n >> 1), it.hk, it.b);
+            }
+            __syncwarp();
+            ++nkv;
+          }
         }
-        // The scores follow their tile's last product on the same issue order,
-        // so they overwrite its probabilities only after they were read.
-        if (u + 1 < tl.count && tl.sees(x, tl.key0(u + 1))) {
-          ok = wait_kv(2 * u + 2);
-          if (ok && !got_q[x]) ok = got_q[x] = mbar_wait_warp(&bars[B_Q + x], 0, abort_flag);
-          if (!ok) break;
-          score(x, u + 1);
+      } else if (warp == kMmaWarp) {
+        // -------------------------------------------- MMA issue (the whole warp; elect.sync inside)
+        constexpr uint32_t kBf16 = Cvt<T>::kIsBf16;
+        constexpr uint32_t id_s = idesc_f16(128, 128, kBf16, 0, 0), id_o = idesc_f16(128, D, kBf16, 0, 1);
+        auto wait_kv = [&](uint32_t n) { return mbar_wait_warp(&full[n % L::stages], (n / L::stages) & 1, abort_flag); };
+        for (int j = 0, i = blockIdx.x; i < P.items && ok; ++j, i += gridDim.x) {
+          if (careful && !(redo[j >> 5] >> (j & 31) & 1)) continue;
+          const Item it = make_item(P, i);
+          if (it.count == 0) continue;
+          const Rows rows0 = it.rows(P, 0), rows1 = it.rows(P, 1);
+          // key tiles of each query tile whose scores, and whose products, are still to be issued
+          int todo_s0 = 0, todo_s1 = 0;
+          for (int u = 0; u < it.count; ++u) {
+            todo_s0 += rows0.sees(it.key0(u));
+            todo_s1 += rows1.sees(it.key0(u));
+          }
+          int todo_p0 = todo_s0, todo_p1 = todo_s1;
+          const int all0 = todo_s0, all1 = todo_s1;
+          for (int u = -1; u < it.count && ok; ++u) {
+            const uint32_t vn = nkv + 2 * u + 1, kn = vn + 1;  // ring slots of this V, the next K
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const Rows& rows = x ? rows1 : rows0;
+              int &todo_s = x ? todo_s1 : todo_s0, &todo_p = x ? todo_p1 : todo_p0;
+              const int all = x ? all1 : all0;
+              const uint32_t nq = x ? nq1 : nq0;
+              uint32_t& ns = x ? ns1 : ns0;
+              if (ok && u >= 0 && rows.sees(it.key0(u))) {
+                const bool fresh = todo_p == all;  // this item's first product: O is written, not added to
+                ok = wait_kv(vn) && mbar_wait_warp(&bars[B_P + x], ns & 1, abort_flag);
+                // the last item's output must have left O
+                if (ok && fresh && nq > 0) ok = mbar_wait_warp(&bars[B_OE + x], (nq - 1) & 1, abort_flag);
+                if (!ok) continue;
+                tc_fence_after();
+                const uint32_t v = sb + L::kv + (vn % L::stages) * L::tile;
+                const bool skip = skip_pv[x] != 0;
+                auto product = [&](int half) {
+#pragma unroll
+                  for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                    mma_f16_ts_warp(tmem + kTmO + x * 128, tmem + kTmS + x * 128 + kk * 8,
+                                    sdesc(v + kk * 2048, 16384, 1024, kSw128), id_o, !fresh || kk > 0);
+                };
+                if (!skip) product(0);
+                ok = mbar_wait_warp(&bars[B_P + 2 + x], ns & 1, abort_flag);
+                if (!ok) continue;
+                ++ns;
+                tc_fence_after();
+                if (!skip) product(1);
+                if (--todo_p == 0) mma_commit_warp(&bars[B_O + x]);
+              }
+              // The scores follow their tile's last product in issue order, so
+              // they overwrite its probabilities only after they were read.
+              if (ok && u + 1 < it.count && rows.sees(it.key0(u + 1))) {
+                ok = wait_kv(kn);
+                if (ok && todo_s == all) ok = mbar_wait_warp(&bars[B_Q + x], nq & 1, abort_flag);
+                if (!ok) continue;
+                const uint32_t q = sb + L::q + x * L::tile, k = sb + L::kv + (kn % L::stages) * L::tile;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                  mma_f16_ss_warp(tmem + kTmS + x * 128, sdesc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024, kSw128),
+                                  sdesc(k + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024, kSw128), id_s, kk > 0);
+                mma_commit_warp(&bars[B_S + x]);
+                if (--todo_s == 0) mma_commit_warp(&bars[B_QE + x]);
+              }
+            }
+            if (ok) {
+              if (u >= 0) mma_commit_warp(&empty[vn % L::stages]);
+              if (u + 1 < it.count) mma_commit_warp(&empty[kn % L::stages]);
+            }
+          }
+          nkv += 2 * it.count;
+          nq0 += rows0.used();
+          nq1 += rows1.used();
         }
       }
-      if (ok) {
-        if (u >= 0) mma_commit_warp(&empty[(2 * u + 1) % L::stages]);
-        if (u + 1 < tl.count) mma_commit_warp(&empty[(2 * u + 2) % L::stages]);
-      }
-    }
-    mma_commit_warp(&bars[B_O]);
-    mma_commit_warp(&bars[B_O + 1]);
-    volatile int never = 0;
-    mbar_wait(&bars[B_O], 0, &never);
-  }
+    } while (careful = again(careful), careful);
   } else {
     regs_more<216>();
     // ------------------------------------------------ softmax: thread = one query row of tile x
@@ -358,136 +491,196 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     // group's barriers still meet.
     const int x = warp >> 2;
     const int r = tid & 127;
-    const int p = tl.p0[x] + r;
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tm_s = tmem + lane_base + kTmS + x * 128, tm_o = tmem + lane_base + kTmO + x * 128;
     const float sl2 = P.scale_log2;
-    const int last = p < len ? p : -1;  // the last visible key; rows behind the sequence see none
-    float m = -INFINITY, l = 0.f;       // running reference maximum (raw scores) and sum
-    bool ok = true, first = true;
-    uint32_t ns = 0;
-    for (int u = 0; u < tl.count; ++u) {
-      const int k0 = tl.key0(u);
-      if (!tl.sees(x, k0)) continue;
-      const bool cut = !tl.whole(x, k0);
-      if (ok) ok = mbar_wait_warp(&bars[B_S + x], ns & 1, abort_flag);
-      ++ns;
-      if (ok) {
-        tc_fence_after();
-        float s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32w(tm_s + c * 32, s + c * 32);
-        if (cut) {
-          const int hi = last - k0, lo = p - P.window + 1 - k0, sk = P.sinks - k0;
-#pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (!(c <= hi && (c >= lo || c < sk))) s[c] = -INFINITY;
-        }
-        float mt = s[0];
-#pragma unroll
-        for (int c = 1; c < 128; ++c) mt = fmaxf(mt, s[c]);
-        // The reference follows the maximum only when a probability would pass
-        // 2^8: most tiles then leave O as it is.
-        float corr = 1.f;
-        if ((mt - m) * sl2 > 8.f || (m == -INFINITY && mt > m)) {
-          corr = m == -INFINITY ? 0.f : fast_exp2((m - mt) * sl2);
-          m = mt;
-          l *= corr;
-        }
-        if (!first && __any_sync(0xffffffffu, corr != 1.f)) {
-          for (int c = 0; c < D; c += 32) {
-            float o[32];
-            uint32_t ou[32];
-            tmem_ld32w(tm_o + c, o);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) ou[i] = __float_as_uint(o[i] * corr);
-            tmem_st32(tm_o + c, ou);
+    do {
+#pragma unroll 1
+      for (int j = 0, i = blockIdx.x; i < P.items; ++j, i += gridDim.x) {
+        if (careful && !(redo[j >> 5] >> (j & 31) & 1)) continue;
+        const Item it = make_item(P, i);
+        const Rows rows = it.rows(P, x);
+        const bool exists = it.row(P, x) + r < P.T;
+        if (!rows.used()) {
+          if (exists) {
+            T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_t * (long long)(it.row(P, x) + r) + P.so_h * it.head(P, x);
+            for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(op)[c] = make_uint4(0, 0, 0, 0);
           }
+          nkv += 2 * it.count;
+          continue;
         }
-        const float ms = m == -INFINITY ? 0.f : m * sl2;
-        float sum0 = 0.f, sum1 = 0.f;
+        const int p = rows.p0 + r;
+        const int last = p < it.len ? p : -1;  // the last visible key; rows behind the sequence see none
+        float m = -INFINITY, l = 0.f;          // running reference maximum (raw scores) and sum
+        bool first = true;
+#pragma unroll 1
+        for (int u = 0; u < it.count; ++u) {
+          const int k0 = it.key0(u);
+          if (!rows.sees(k0)) continue;
+          const bool cut = !rows.whole(k0);
+          if (ok) ok = mbar_wait_warp(&bars[B_S + x], ns0 & 1, abort_flag);
+          ++ns0;
+          if (ok) {
+            tc_fence_after();
+            float s[128];
+            tmem_ld64w(tm_s, s);
+            tmem_ld64w(tm_s + 64, s + 64);
+            if (cut) mask_row(s, last - k0, p - P.window + 1 - k0, P.sinks - k0);
+            float mx[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
+            for (int c = 0; c < 8; ++c) mx[c] = fmaxf(s[c], s[c + 8]);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const float e0 = fast_exp2(fmaf(s[64 * h + 2 * c], sl2, -ms));
-            const float e1 = fast_exp2(fmaf(s[64 * h + 2 * c + 1], sl2, -ms));
-            sum0 += e0;
-            sum1 += e1;
-            pk[c] = Cvt<T>::pack(e0, e1);
-          }
-          tmem_st32(tm_s + 32 * h, pk);
-        }
-        l += sum0 + sum1;
-        tmem_wait_st();
-      }
-      bool slow = false;
-      if (cut) {
-        const int i = 2 * u + 1;
-        const uint8_t* vt = sm + L::kv + (i % L::stages) * L::tile;
-        if (ok) ok = mbar_wait_warp(&full[i % L::stages], (i / L::stages) & 1, abort_flag);
-        bool bad = false;
-        if (ok) {
-          // one key per thread; a value that is not finite times 0 is NaN
-          using V2 = typename Pair<T>::V;
-          V2 acc = Pair<T>::zero();
-          for (uint32_t c = 0; c < L::boxes * 8; ++c) {
-            const uint4 w = *reinterpret_cast<const uint4*>(vt + (c >> 3) * 16384 + sw128_off(r, c & 7));
-            acc = __hfma2(*reinterpret_cast<const V2*>(&w.x), Pair<T>::zero(), acc);
-            acc = __hfma2(*reinterpret_cast<const V2*>(&w.y), Pair<T>::zero(), acc);
-            acc = __hfma2(*reinterpret_cast<const V2*>(&w.z), Pair<T>::zero(), acc);
-            acc = __hfma2(*reinterpret_cast<const V2*>(&w.w), Pair<T>::zero(), acc);
-          }
-          const float z = __low2float(acc) + __high2float(acc);
-          bad = z != z;
-        }
-        slow = bar_any(1 + x, 128, bad);
-        if (slow && ok) sum_visible<T, D>(tm_s, tm_o, vt, first, k0, last, p - P.window, P.sinks);
-      }
-      first = false;
-      if (ok) {
-        tc_fence_before();
-        if (lane == 0) {
-          if ((warp & 3) == 0) skip_pv[x] = slow;
-          __threadfence_block();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[B_P + x]);
-      }
-    }
-    // ------------------------------------------------ o = O / l
-    if (ok && tl.count > 0) ok = mbar_wait_warp(&bars[B_O + x], 0, abort_flag);
-    if (ok) {
-      tc_fence_after();
-      const int i = row0 + (P.pair_heads ? 0 : x * kTile) + r;
-      const int h = hy + (P.pair_heads ? x : 0);
-      const bool dead = first || last < 0;
-      const float inv = dead ? 0.f : 1.f / l;
-      T* op = static_cast<T*>(P.o) + P.so_b * b + P.so_t * (long long)i + P.so_h * h;
-      for (int c = 0; c < D; c += 32) {
-        float o[32];
-        tmem_ld32w(tm_o + c, o);
-        if (i < P.T) {
+            for (int c = 16; c < 128; c += 16)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 w;
-            uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+              for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], fmaxf(s[c + e], s[c + 8 + e]));
+            const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                   fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+            // The reference follows the maximum only when a probability would
+            // pass 2^8: most tiles then leave O as it is.
+            const bool up = (mt - m) * sl2 > 8.f || (m == -INFINITY && mt > m);
+            if (__any_sync(0xffffffffu, up)) {
+              const float corr = !up ? 1.f : (m == -INFINITY ? 0.f : fast_exp2((m - mt) * sl2));
+              if (up) m = mt;
+              l *= corr;
+              if (!first) {
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                  float o[16];
+                  tmem_ld16w(tm_o + c, o);
+                  uint32_t ou[16];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float a = o[8 * j + 2 * e] * inv, c2 = o[8 * j + 2 * e + 1] * inv;
-              wp[e] = dead ? 0u : Cvt<T>::pack(a, c2);
+                  for (int e = 0; e < 16; ++e) ou[e] = __float_as_uint(o[e] * corr);
+                  tmem_st16(tm_o + c, ou);
+                }
+              }
             }
-            reinterpret_cast<uint4*>(op + c)[j] = w;
+            const float ms = m == -INFINITY ? 0.f : m * sl2;
+            const F2 sl = f2(sl2, sl2), nm = f2(-ms, -ms);
+            F2 sum0 = f2(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+            for (int qt = 0; qt < 4; ++qt) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                float2 e = f2_get(f2_fma(f2(s[32 * qt + 2 * c], s[32 * qt + 2 * c + 1]), sl, nm));
+                e = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                if (c & 1)
+                  sum1 = f2_add(sum1, f2(e.x, e.y));
+                else
+                  sum0 = f2_add(sum0, f2(e.x, e.y));
+                pk[c] = Cvt<T>::pack(e.x, e.y);
+              }
+              tmem_st16(tm_s + 16 * qt, pk);
+              if (qt == 1 && !careful) {  // the product's first half starts under the second one's exponentials
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars[B_P + x]);
+              }
+            }
+            const float2 sum = f2_get(f2_add(sum0, sum1));
+            l += sum.x + sum.y;
+            tmem_wait_st();
+          }
+          if (careful) {
+            bool slow = false;
+            if (cut) {
+              const uint32_t vn = nkv + 2 * u + 1;
+              const uint8_t* vt = sm + L::kv + (vn % L::stages) * L::tile;
+              if (ok) ok = mbar_wait_warp(&full[vn % L::stages], (vn / L::stages) & 1, abort_flag);
+              slow = bar_any(1 + x, 128, ok && row_not_finite<T, D>(vt, r));
+              if (slow && ok) sum_visible<T, D>(tm_s, tm_o, vt, first, k0, last, p - P.window, P.sinks);
+            }
+            if (ok && r == 0) skip_pv[x] = slow;
+            __threadfence_block();
+            __syncwarp();
+            if (ok && lane == 0) {
+              tc_fence_before();
+              mbar_arrive(&bars[B_P + x]);
+            }
+          }
+          first = false;
+          if (ok) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[B_P + 2 + x]);
           }
         }
+        // -------------------------------------------- o = O / l
+        if (ok) ok = mbar_wait_warp(&bars[B_O + x], nq0 & 1, abort_flag);
+        if (ok) {
+          tc_fence_after();
+          const bool live = last >= 0;
+          const float inv = 1.f / l;
+          float odd = 0.f;  // NaN if some output is not finite
+          // Rows leave through shared memory, so that a store covers whole lines.
+          uint8_t* stage = sm + L::out + warp * 4096;
+          const int row = it.row(P, x) + (r - lane);  // this warp's first
+          T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_h * it.head(P, x) + P.so_t * (long long)row;
+#pragma unroll 1
+          for (int half = 0; half < D / 64; ++half) {
+            float o[64];
+            tmem_ld64w(tm_o + 64 * half, o);
+            if (half == D / 64 - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars[B_OE + x]);
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint4 w;
+              uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float a = o[8 * c + 2 * e] * inv, b2 = o[8 * c + 2 * e + 1] * inv;
+                odd = fmaf(a, 0.f, odd);
+                odd = fmaf(b2, 0.f, odd);
+                wp[e] = live ? Cvt<T>::pack(a, b2) : 0u;
+              }
+              *reinterpret_cast<uint4*>(stage + sw128_off(lane, c)) = w;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const int rr = 4 * c + (lane >> 3);
+              const uint4 w = *reinterpret_cast<const uint4*>(stage + sw128_off(rr, lane & 7));
+              if (row + rr < P.T) reinterpret_cast<uint4*>(op + P.so_t * (long long)rr + 64 * half)[lane & 7] = w;
+            }
+            __syncwarp();
+          }
+          if (!careful && exists && live && odd != odd) {
+            atomicOr(&redo[j >> 5], 1u << (j & 31));
+            *any_redo = 1;
+          }
+        }
+        ++nq0;
+        nkv += 2 * it.count;
       }
-      tc_fence_before();
-    }
+    } while (careful = again(careful), careful);
+  }
+  // On an abort the loads and products still in flight end before the CTA leaves.
+  if (warp == kTmaWarp && *abort_flag) {
+    volatile int never = 0;
+    if (nq0 > 0) mbar_wait(&bars[B_Q], (nq0 - 1) & 1, &never);
+    if (nq1 > 0) mbar_wait(&bars[B_Q + 1], (nq1 - 1) & 1, &never);
+    for (uint32_t n = nkv > L::stages ? nkv - L::stages : 0; n < nkv; ++n)
+      mbar_wait(&full[n % L::stages], (n / L::stages) & 1, &never);
   }
   __syncthreads();
   if (tid == 0 && *abort_flag && P.status) atomicOr(P.status, 1 << GDN_ERR_TIMEOUT);
   if (warp == kMmaWarp) {
+    if (*abort_flag) {
+      // a commit of its own: every product issued so far has ended when it arrives
+      if (lane == 0) {
+        mbar_init(&bars[B_COUNT], 1);
+        fence_mbar_init();
+      }
+      __syncwarp();
+      mma_commit_warp(&bars[B_COUNT]);
+      volatile int never = 0;
+      mbar_wait(&bars[B_COUNT], 0, &never);
+      __syncwarp();
+    }
     tc_fence_after();
     tmem_dealloc(tmem, kTmCols);
   }
@@ -562,7 +755,17 @@ int run(const gdn_window_attn_args* a, void* stream) {
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.pair_heads = p.G % 2 == 0;
   const int rows = p.pair_heads ? kTile : 2 * kTile;
-  const dim3 grid((a->T + rows - 1) / rows, p.pair_heads ? a->H / 2 : a->H, a->B);
+  p.nx = (a->T + rows - 1) / rows;
+  p.ny = p.pair_heads ? a->H / 2 : a->H;
+  const long long items = (long long)p.nx * p.ny * a->B;
+  if (items > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED;
+  p.items = int(items);
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return cuda_failed();
+  // one CTA per SM, more only where one could not note all its items
+  long long ctas = (items + kMaxItems - 1) / kMaxItems;
+  if (ctas < sms) ctas = items < sms ? items : sms;
+  const dim3 grid{unsigned(ctas)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = a->dtype == GDN_DTYPE_BF16;
   if (a->D == 128)
