@@ -42,14 +42,13 @@ namespace gdn {
 namespace wa {
 namespace {
 
-constexpr int kTile = 128;          // query rows and keys per tile
+constexpr int kTile = 128;          // query rows per tile
+constexpr int kKeys = 64;           // keys per tile
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
-// Three warpgroups, so that registers can be moved between them: 168 each at
-// launch, then 2 x 216 for the softmax warps and 72 for the others (504 in all).
-constexpr int kThreads = 384;
+constexpr int kThreads = 320;
 constexpr int kMaxItems = 8192;     // of one CTA
 constexpr uint32_t kTmCols = 512;
-constexpr uint32_t kTmS = 0, kTmO = 256;  // + 128 x tile
+constexpr uint32_t kTmS = 0, kTmO = 256;  // + 128 x tile (+ 64 x buffer of the scores)
 
 struct Params {
   CUtensorMap tm_q, tm_k, tm_v;
@@ -67,30 +66,60 @@ struct Params {
 template <int D>
 struct Lay {
   static constexpr uint32_t boxes = D / 64;               // 64-column boxes of a tile
-  static constexpr uint32_t tile = boxes * 16384;         // bytes of a 128-row tile
-  static constexpr uint32_t stages = D == 128 ? 4 : 6;
+  static constexpr uint32_t qtile = boxes * 16384, kvtile = boxes * 8192;  // bytes
+  static constexpr uint32_t stages = 8;
   static constexpr uint32_t q = 0;                        // two query tiles
-  static constexpr uint32_t kv = 2 * tile;                // ring of K and V tiles
-  static constexpr uint32_t out = kv + stages * tile;      // [8 warps][32 rows][64 columns] of outputs
+  static constexpr uint32_t kv = 2 * qtile;               // ring of K and V tiles
+  static constexpr uint32_t out = kv + stages * kvtile;      // [8 warps][32 rows][64 columns] of outputs
   static constexpr uint32_t bars = out + 32768;
-  static constexpr uint32_t misc = bars + 8 * (2 * stages + 16);
+  static constexpr uint32_t misc = bars + 8 * (2 * stages + 20);
   static constexpr uint32_t redo = misc + 64;             // one bit per item of this CTA
   static constexpr uint32_t bytes = redo + kMaxItems / 8;
   static constexpr uint32_t alloc = bytes + 1024;
 };
 
-// Barriers behind the ring's full[stages], empty[stages]; two each, one per tile.
-// B_P: the first and, two on, the second half of the probabilities.
-enum { B_Q = 0, B_QE = 2, B_S = 4, B_P = 6, B_O = 10, B_OE = 12, B_COUNT = 14 };
+// Barriers behind the ring's full[stages], empty[stages]; two each, one per query
+// tile, or four, one per tile and score buffer.
+// Upper half of the operands' shared-memory descriptors: 1024 bytes between groups
+// of 8 rows, descriptor version 1, 128-byte swizzle.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (uint32_t(kSw128) << 29);
+enum { B_Q = 0, B_QE = 2, B_S = 4, B_P = 8, B_V = 12, B_O = 14, B_OE = 16, B_COUNT = 18 };
 
-__device__ __forceinline__ void mma_f16_ts_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                                uint32_t accumulate) {
+// Four K = 16 steps of a product, issued by one elected lane of the converged
+// warp.  The descriptors' upper halves are constants and their lower halves
+// advance by constants, so that a step costs a few instructions: with two busy
+// softmax warps beside it the issuing warp is what the products wait for first.
+__device__ __forceinline__ void mma4_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                        uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, e, t;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tsetp.eq.b32 t, 0, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t"
+      "add.u32 x, %1, 2;\n\tadd.u32 y, %3, 2;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, t;\n\t"
+      "add.u32 x, %1, 4;\n\tadd.u32 y, %3, 4;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, t;\n\t"
+      "add.u32 x, %1, 6;\n\tadd.u32 y, %3, 6;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, t;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A from TMEM (8 columns a step), B with its steps 2048 bytes apart.
+__device__ __forceinline__ void mma4_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e, t;\n\t.reg .b64 b;\n\t.reg .b32 x, y;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t"
+      "add.u32 x, %1, 8;\n\tadd.u32 y, %2, 128;\n\tmov.b64 b, {y, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %4, t;\n\t"
+      "add.u32 x, %1, 16;\n\tadd.u32 y, %2, 256;\n\tmov.b64 b, {y, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %4, t;\n\t"
+      "add.u32 x, %1, 24;\n\tadd.u32 y, %2, 384;\n\tmov.b64 b, {y, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %4, t;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -158,9 +187,6 @@ __device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
   return r;
 }
 
-template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
 template <typename T> struct Pair;
 template <> struct Pair<__half> {
   static __device__ __forceinline__ __half2 zero() { return __floats2half2_rn(0.f, 0.f); }
@@ -178,15 +204,21 @@ struct Rows {
 
   // whether it has a row that sees anything (then its first row sees itself)
   __device__ __forceinline__ bool used() const { return p1 >= p0 && p0 < len; }
-  // whether some row sees a key of the tile at k0
-  __device__ __forceinline__ bool sees(int k0) const {
-    return used() && k0 < len && k0 <= p1 && (k0 < sinks || k0 + kTile > p0 - window + 1);
-  }
   // whether every row sees every key of the tile at k0
   __device__ __forceinline__ bool whole(int k0) const {
-    const int k1 = k0 + kTile - 1;
+    const int k1 = k0 + kKeys - 1;
     return k1 <= p0 && k1 < len && (k1 < sinks || p1 - k0 < window);
   }
+};
+
+// The key tiles, by their order in an item, that one query tile sees: some of the
+// sinks' first, then a run of the window's.
+struct Seen {
+  int sinks, from, to;
+  __device__ __forceinline__ bool operator()(int u) const { return u >= 0 && u <= to && (u < sinks || u >= from); }
+  __device__ __forceinline__ int tiles() const { return to < 0 ? 0 : sinks + (to - from + 1); }
+  __device__ __forceinline__ int first() const { return sinks > 0 ? 0 : from; }
+  __device__ __forceinline__ int last() const { return to; }
 };
 
 // A work item and its key tiles, in order: those of the sinks, then those of the window.
@@ -194,9 +226,18 @@ struct Rows {
 // with this much shared memory taken, that means L2.)
 struct Item {
   int b, hy, hk, row0;  // hy: the (first) query head
-  int len, n_sink, w0, count;
+  int len, count;
+  int sink_tiles;  // key tiles that hold sinks
+  int n_sink, w0;  // order: tiles 0 .. n_sink - 1, then w0, w0 + 1 ...
 
-  __device__ __forceinline__ int key0(int u) const { return (u < n_sink ? u : w0 + (u - n_sink)) * kTile; }
+  __device__ __forceinline__ int key0(int u) const { return (u < n_sink ? u : w0 + (u - n_sink)) * kKeys; }
+  // (The first row that a query tile has sees itself, so there always is a run of the window's.)
+  __device__ __forceinline__ Seen seen(const Rows& r) const {
+    if (!r.used()) return Seen{0, 0, -1};
+    const int lo = r.p0 - r.window + 1;
+    const int from = (lo > 0 ? lo / kKeys : 0) - w0 + n_sink, to = (r.p1 < len ? r.p1 : len - 1) / kKeys - w0 + n_sink;
+    return Seen{sink_tiles < from ? sink_tiles : from, from, to};
+  }
   __device__ __forceinline__ int row(const Params& P, int x) const { return row0 + (P.pair_heads ? 0 : x * kTile); }
   __device__ __forceinline__ int head(const Params& P, int x) const { return hy + (P.pair_heads ? x : 0); }
   __device__ __forceinline__ Rows rows(const Params& P, int x) const {
@@ -214,19 +255,19 @@ __device__ __forceinline__ Item make_item(const Params& P, int i) {
   it.hk = it.hy / P.G;
   it.len = P.S;
   if (P.lengths) {
-    it.len = P.lengths[it.b];
+    it.len = __shfl_sync(0xffffffffu, P.lengths[it.b], 0);
     it.len = it.len < 0 ? 0 : (it.len > P.S ? P.S : it.len);
   }
   const Rows r0 = it.rows(P, 0), r1 = it.rows(P, 1);
   int end = r1.p1 > r0.p1 ? r1.p1 : r0.p1;
   if (end > it.len - 1) end = it.len - 1;
+  it.sink_tiles = P.sinks > 0 ? (P.sinks - 1) / kKeys + 1 : 0;
   it.n_sink = it.w0 = it.count = 0;
   if (r0.p0 >= it.len) return it;
   const int lo = r0.p0 - P.window + 1;
-  it.n_sink = P.sinks > 0 ? (P.sinks - 1) / kTile + 1 : 0;
-  it.w0 = lo > 0 ? lo / kTile : 0;
-  if (it.n_sink >= it.w0) it.n_sink = it.w0;  // the sinks' tiles run into the window's
-  it.count = it.n_sink + (end / kTile - it.w0 + 1);
+  it.w0 = lo > 0 ? lo / kKeys : 0;
+  it.n_sink = it.sink_tiles < it.w0 ? it.sink_tiles : it.w0;  // w0: the sinks' tiles run into the window's
+  it.count = it.n_sink + (end / kKeys - it.w0 + 1);
   return it;
 }
 
@@ -254,7 +295,7 @@ __device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uin
     } else {
       tmem_ld32w(tm_o + c0, o);
     }
-    for (int j = 0; j < kTile; ++j) {
+    for (int j = 0; j < kKeys; ++j) {
       const float2 pp = Cvt<T>::unpack(tmem_ld1w(tm_p + (j >> 1)));
       const float pj = (j & 1) ? pp.y : pp.x;
       const int kj = k0 + j;
@@ -262,7 +303,7 @@ __device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uin
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint4 w =
-              *reinterpret_cast<const uint4*>(vt + (c0 >> 6) * 16384 + sw128_off(j, ((c0 & 63) >> 3) + i));
+              *reinterpret_cast<const uint4*>(vt + (c0 >> 6) * 8192 + sw128_off(j, ((c0 & 63) >> 3) + i));
           const float2 a = Cvt<T>::unpack(w.x), b = Cvt<T>::unpack(w.y), c = Cvt<T>::unpack(w.z),
                        d = Cvt<T>::unpack(w.w);
           o[8 * i] = fmaf(pj, a.x, o[8 * i]);
@@ -287,7 +328,7 @@ __device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uin
 // Masked scores of one tile: this row's visible keys are those up to hi, from lo on or below sk.
 __device__ __forceinline__ void mask_row(float* s, int hi, int lo, int sk) {
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < kKeys / 32; ++w) {
     // bits of the 32 columns from 32 w on
     auto below = [&](int n) {  // columns < n
       n -= 32 * w;
@@ -306,7 +347,7 @@ __device__ __noinline__ bool row_not_finite(const uint8_t* vt, int r) {
   using V2 = typename Pair<T>::V;
   V2 acc = Pair<T>::zero();
   for (int c = 0; c < D / 8; ++c) {
-    const uint4 w = *reinterpret_cast<const uint4*>(vt + (c >> 3) * 16384 + sw128_off(r, c & 7));
+    const uint4 w = *reinterpret_cast<const uint4*>(vt + (c >> 3) * 8192 + sw128_off(r, c & 7));
     acc = __hfma2(*reinterpret_cast<const V2*>(&w.x), Pair<T>::zero(), acc);
     acc = __hfma2(*reinterpret_cast<const V2*>(&w.y), Pair<T>::zero(), acc);
     acc = __hfma2(*reinterpret_cast<const V2*>(&w.z), Pair<T>::zero(), acc);
@@ -326,10 +367,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   uint64_t* bars = empty + L::stages;
   uint32_t* tmem_base_p = reinterpret_cast<uint32_t*>(sm + L::misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::misc + 4);
-  volatile int* skip_pv = reinterpret_cast<volatile int*>(sm + L::misc + 8);  // [2]: the product is already in O
-  volatile int* any_redo = reinterpret_cast<volatile int*>(sm + L::misc + 16);
+  volatile int* skip_pv = reinterpret_cast<volatile int*>(sm + L::misc + 8);  // per score buffer: its product is already in O
+  volatile int* any_redo = reinterpret_cast<volatile int*>(sm + L::misc + 24);
   uint32_t* redo = reinterpret_cast<uint32_t*>(sm + L::redo);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be uniform: roles may use uniform registers
   const uint32_t sb = smem_u32(sm);
 
   if (tid == 0) {
@@ -337,18 +379,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(&bars[B_Q + x], 1);
-      mbar_init(&bars[B_QE + x], 1);
-      mbar_init(&bars[B_S + x], 1);
-      mbar_init(&bars[B_P + x], 4);
-      mbar_init(&bars[B_P + 2 + x], 4);
-      mbar_init(&bars[B_O + x], 1);
-      mbar_init(&bars[B_OE + x], 4);
+    for (int i = 0; i < B_COUNT; ++i) {
+      const bool softmax = (i >= B_P && i < B_P + 4) || i >= B_OE;  // arrived at by a group's four warps
+      mbar_init(&bars[i], softmax ? 4 : 1);
     }
     *abort_flag = 0;
     *any_redo = 0;
-    skip_pv[0] = skip_pv[1] = 0;
+    for (int i = 0; i < 4; ++i) skip_pv[i] = 0;
     fence_mbar_init();
   }
   for (int i = tid; i < kMaxItems / 32; i += kThreads) redo[i] = 0;
@@ -358,7 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   }
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_base_p;
+  // All 512 columns are this CTA's, so they start at 0: a constant.
+  constexpr uint32_t tmem = 0;
 
   // A second, careful pass follows if the first one noted any item; all warps meet in between.
   auto again = [&](bool careful) {
@@ -368,11 +406,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   // Counts over all items and passes, for the barriers' phases:
   uint32_t nkv = 0;           // ring slots used
   uint32_t nq0 = 0, nq1 = 0;  // items that used query tile 0, 1 (softmax: the first for its own)
-  uint32_t ns0 = 0, ns1 = 0;  // key tiles of query tile 0, 1 (the same)
+  uint32_t ns0 = 0, ns1 = 0;  // key tiles of query tile 0, 1 (the same): scores
+  uint32_t np0 = 0, np1 = 0;  // and products
   bool ok = true, careful = false;
 
   if (warp >= 8) {
-    regs_less<72>();
     do {
       if (warp == kTmaWarp) {
         // -------------------------------------------- producer: Q tiles, then K0 V0 K1 V1 ...
@@ -386,9 +424,9 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
             if (nq > 0) ok = mbar_wait_warp(&bars[B_QE + x], (nq - 1) & 1, abort_flag);
             if (!ok) continue;
             if (lane == 0) {
-              mbar_arrive_expect_tx(&bars[B_Q + x], L::tile);
+              mbar_arrive_expect_tx(&bars[B_Q + x], L::qtile);
               for (uint32_t c = 0; c < L::boxes; ++c)
-                tma_load_4d(sm + L::q + x * L::tile + c * 16384, &P.tm_q, &bars[B_Q + x], c * 64, it.row(P, x),
+                tma_load_4d(sm + L::q + x * L::qtile + c * 16384, &P.tm_q, &bars[B_Q + x], c * 64, it.row(P, x),
                             it.head(P, x), it.b);
             }
             __syncwarp();
@@ -399,9 +437,9 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
             if (nkv >= L::stages) ok = mbar_wait_warp(&empty[s], (nkv / L::stages - 1) & 1, abort_flag);
             if (!ok) break;
             if (lane == 0) {
-              mbar_arrive_expect_tx(&full[s], L::tile);
+              mbar_arrive_expect_tx(&full[s], L::kvtile);
               for (uint32_t c = 0; c < L::boxes; ++c)
-                tma_load_4d(sm + L::kv + s * L::tile + c * 16384, (n & 1) ? &P.tm_v : &P.tm_k, &full[s], c * 64,
+                tma_load_4d(sm + L::kv + s * L::kvtile + c * 8192, (n & 1) ? &P.tm_v : &P.tm_k, &full[s], c * 64,
                             it.key0(n >> 1), it.hk, it.b);
             }
             __syncwarp();
@@ -411,71 +449,62 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       } else if (warp == kMmaWarp) {
         // -------------------------------------------- MMA issue (the whole warp; elect.sync inside)
         constexpr uint32_t kBf16 = Cvt<T>::kIsBf16;
-        constexpr uint32_t id_s = idesc_f16(128, 128, kBf16, 0, 0), id_o = idesc_f16(128, D, kBf16, 0, 1);
+        constexpr uint32_t id_s = idesc_f16(128, kKeys, kBf16, 0, 0), id_o = idesc_f16(128, D, kBf16, 0, 1);
         auto wait_kv = [&](uint32_t n) { return mbar_wait_warp(&full[n % L::stages], (n / L::stages) & 1, abort_flag); };
         for (int j = 0, i = blockIdx.x; i < P.items && ok; ++j, i += gridDim.x) {
           if (careful && !(redo[j >> 5] >> (j & 31) & 1)) continue;
           const Item it = make_item(P, i);
           if (it.count == 0) continue;
           const Rows rows0 = it.rows(P, 0), rows1 = it.rows(P, 1);
-          // key tiles of each query tile whose scores, and whose products, are still to be issued
-          int todo_s0 = 0, todo_s1 = 0;
-          for (int u = 0; u < it.count; ++u) {
-            todo_s0 += rows0.sees(it.key0(u));
-            todo_s1 += rows1.sees(it.key0(u));
-          }
-          int todo_p0 = todo_s0, todo_p1 = todo_s1;
-          const int all0 = todo_s0, all1 = todo_s1;
-          for (int u = -1; u < it.count && ok; ++u) {
-            const uint32_t vn = nkv + 2 * u + 1, kn = vn + 1;  // ring slots of this V, the next K
+          const Seen seen0 = it.seen(rows0), seen1 = it.seen(rows1);
+          int left0 = seen0.tiles(), left1 = seen1.tiles();  // products still to be issued
+          const int last0 = seen0.last(), last1 = seen1.last(), first0 = seen0.first(), first1 = seen1.first();
+          // Scores run two key tiles ahead of the products, so that a softmax group
+          // finds its next tile's ready.
+          for (int u = -2; u < it.count && ok; ++u) {
+            const uint32_t vs = (nkv + 2 * u + 1) % L::stages, ks = (nkv + 2 * u + 4) % L::stages;
+            const uint32_t v_lo = ((sb + L::kv + vs * L::kvtile) >> 4) | (512u << 16);  // 8192 bytes between its boxes
+            const uint32_t k_lo = ((sb + L::kv + ks * L::kvtile) >> 4) | (1u << 16);
+            if (u >= 0) ok = wait_kv(nkv + 2 * u + 1);
+            if (ok && u + 2 < it.count) ok = wait_kv(nkv + 2 * u + 4);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const Rows& rows = x ? rows1 : rows0;
-              int &todo_s = x ? todo_s1 : todo_s0, &todo_p = x ? todo_p1 : todo_p0;
-              const int all = x ? all1 : all0;
+              const Seen& seen = x ? seen1 : seen0;
+              int& left = x ? left1 : left0;
               const uint32_t nq = x ? nq1 : nq0;
-              uint32_t& ns = x ? ns1 : ns0;
-              if (ok && u >= 0 && rows.sees(it.key0(u))) {
-                const bool fresh = todo_p == all;  // this item's first product: O is written, not added to
-                ok = wait_kv(vn) && mbar_wait_warp(&bars[B_P + x], ns & 1, abort_flag);
+              uint32_t &ns = x ? ns1 : ns0, &np = x ? np1 : np0;
+              if (ok && seen(u)) {
+                const bool fresh = u == (x ? first1 : first0);  // this item's first product: O is written, not added to
+                const uint32_t buf = np & 1;
+                ok = mbar_wait_warp(&bars[B_P + 2 * x + buf], (np >> 1) & 1, abort_flag);
                 // the last item's output must have left O
                 if (ok && fresh && nq > 0) ok = mbar_wait_warp(&bars[B_OE + x], (nq - 1) & 1, abort_flag);
                 if (!ok) continue;
+                ++np;
                 tc_fence_after();
-                const uint32_t v = sb + L::kv + (vn % L::stages) * L::tile;
-                const bool skip = skip_pv[x] != 0;
-                auto product = [&](int half) {
-#pragma unroll
-                  for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                    mma_f16_ts_warp(tmem + kTmO + x * 128, tmem + kTmS + x * 128 + kk * 8,
-                                    sdesc(v + kk * 2048, 16384, 1024, kSw128), id_o, !fresh || kk > 0);
-                };
-                if (!skip) product(0);
-                ok = mbar_wait_warp(&bars[B_P + 2 + x], ns & 1, abort_flag);
-                if (!ok) continue;
-                ++ns;
-                tc_fence_after();
-                if (!skip) product(1);
-                if (--todo_p == 0) mma_commit_warp(&bars[B_O + x]);
+                if (!careful || !skip_pv[2 * x + buf])
+                  mma4_ts(tmem + kTmO + x * 128, tmem + kTmS + x * 128 + buf * 64, v_lo, kDescHi, id_o, !fresh);
+                mma_commit_warp(&bars[B_V + x]);
+                if (--left == 0) mma_commit_warp(&bars[B_O + x]);
               }
-              // The scores follow their tile's last product in issue order, so
-              // they overwrite its probabilities only after they were read.
-              if (ok && u + 1 < it.count && rows.sees(it.key0(u + 1))) {
-                ok = wait_kv(kn);
-                if (ok && todo_s == all) ok = mbar_wait_warp(&bars[B_Q + x], nq & 1, abort_flag);
+              // A score buffer is written again two tiles on: in issue order after the
+              // product that read its probabilities.
+              if (ok && seen(u + 2)) {
+                if (u + 2 == (x ? first1 : first0)) ok = mbar_wait_warp(&bars[B_Q + x], nq & 1, abort_flag);
                 if (!ok) continue;
-                const uint32_t q = sb + L::q + x * L::tile, k = sb + L::kv + (kn % L::stages) * L::tile;
+                const uint32_t q_lo = ((sb + L::q + x * L::qtile) >> 4) | (1u << 16);
+                const uint32_t buf = ns & 1;
+                ++ns;
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk)
-                  mma_f16_ss_warp(tmem + kTmS + x * 128, sdesc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024, kSw128),
-                                  sdesc(k + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024, kSw128), id_s, kk > 0);
-                mma_commit_warp(&bars[B_S + x]);
-                if (--todo_s == 0) mma_commit_warp(&bars[B_QE + x]);
+                for (uint32_t c = 0; c < L::boxes; ++c)
+                  mma4_ss(tmem + kTmS + x * 128 + buf * 64, q_lo + c * 1024, kDescHi, k_lo + c * 512, kDescHi, id_s, c);
+                mma_commit_warp(&bars[B_S + 2 * x + buf]);
+                if (u + 2 == (x ? last1 : last0)) mma_commit_warp(&bars[B_QE + x]);
               }
             }
             if (ok) {
-              if (u >= 0) mma_commit_warp(&empty[vn % L::stages]);
-              if (u + 1 < it.count) mma_commit_warp(&empty[kn % L::stages]);
+              if (u >= 0) mma_commit_warp(&empty[vs]);
+              if (u + 2 < it.count) mma_commit_warp(&empty[ks]);
             }
           }
           nkv += 2 * it.count;
@@ -485,14 +514,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       }
     } while (careful = again(careful), careful);
   } else {
-    regs_more<216>();
     // ------------------------------------------------ softmax: thread = one query row of tile x
     // After an abort a warp runs on without waiting or computing, so that the
     // group's barriers still meet.
     const int x = warp >> 2;
     const int r = tid & 127;
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t tm_s = tmem + lane_base + kTmS + x * 128, tm_o = tmem + lane_base + kTmO + x * 128;
+    const uint32_t tm_s0 = tmem + lane_base + kTmS + x * 128, tm_o = tmem + lane_base + kTmO + x * 128;
     const float sl2 = P.scale_log2;
     do {
 #pragma unroll 1
@@ -509,28 +537,30 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           nkv += 2 * it.count;
           continue;
         }
+        const Seen seen = it.seen(rows);
         const int p = rows.p0 + r;
         const int last = p < it.len ? p : -1;  // the last visible key; rows behind the sequence see none
         float m = -INFINITY, l = 0.f;          // running reference maximum (raw scores) and sum
         bool first = true;
 #pragma unroll 1
         for (int u = 0; u < it.count; ++u) {
+          if (!seen(u)) continue;
           const int k0 = it.key0(u);
-          if (!rows.sees(k0)) continue;
           const bool cut = !rows.whole(k0);
-          if (ok) ok = mbar_wait_warp(&bars[B_S + x], ns0 & 1, abort_flag);
+          const uint32_t buf = ns0 & 1, before = (ns0 - 1) & 1;
+          const uint32_t tm_s = tm_s0 + buf * 64;
+          if (ok) ok = mbar_wait_warp(&bars[B_S + 2 * x + buf], (ns0 >> 1) & 1, abort_flag);
           ++ns0;
           if (ok) {
             tc_fence_after();
-            float s[128];
+            float s[kKeys];
             tmem_ld64w(tm_s, s);
-            tmem_ld64w(tm_s + 64, s + 64);
             if (cut) mask_row(s, last - k0, p - P.window + 1 - k0, P.sinks - k0);
             float mx[8];
 #pragma unroll
             for (int c = 0; c < 8; ++c) mx[c] = fmaxf(s[c], s[c + 8]);
 #pragma unroll
-            for (int c = 16; c < 128; c += 16)
+            for (int c = 16; c < kKeys; c += 16)
 #pragma unroll
               for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], fmaxf(s[c + e], s[c + 8 + e]));
             const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
@@ -543,14 +573,19 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
               if (up) m = mt;
               l *= corr;
               if (!first) {
+                // the product before has to be in O
+                ok = mbar_wait_warp(&bars[B_V + x], before, abort_flag);
+                if (ok) {
+                  tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < D; c += 16) {
-                  float o[16];
-                  tmem_ld16w(tm_o + c, o);
-                  uint32_t ou[16];
+                  for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    tmem_ld32w(tm_o + c, o);
+                    uint32_t ou[32];
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) ou[e] = __float_as_uint(o[e] * corr);
-                  tmem_st16(tm_o + c, ou);
+                    for (int e = 0; e < 32; ++e) ou[e] = __float_as_uint(o[e] * corr);
+                    tmem_st32(tm_o + c, ou);
+                  }
                 }
               }
             }
@@ -558,11 +593,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
             const F2 sl = f2(sl2, sl2), nm = f2(-ms, -ms);
             F2 sum0 = f2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
-            for (int qt = 0; qt < 4; ++qt) {
+            for (int h = 0; h < 2; ++h) {
               uint32_t pk[16];
 #pragma unroll
               for (int c = 0; c < 16; ++c) {
-                float2 e = f2_get(f2_fma(f2(s[32 * qt + 2 * c], s[32 * qt + 2 * c + 1]), sl, nm));
+                float2 e = f2_get(f2_fma(f2(s[32 * h + 2 * c], s[32 * h + 2 * c + 1]), sl, nm));
                 e = make_float2(fast_exp2(e.x), fast_exp2(e.y));
                 if (c & 1)
                   sum1 = f2_add(sum1, f2(e.x, e.y));
@@ -570,13 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
                   sum0 = f2_add(sum0, f2(e.x, e.y));
                 pk[c] = Cvt<T>::pack(e.x, e.y);
               }
-              tmem_st16(tm_s + 16 * qt, pk);
-              if (qt == 1 && !careful) {  // the product's first half starts under the second one's exponentials
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars[B_P + x]);
-              }
+              tmem_st16(tm_s + 16 * h, pk);
             }
             const float2 sum = f2_get(f2_add(sum0, sum1));
             l += sum.x + sum.y;
@@ -586,24 +615,23 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
             bool slow = false;
             if (cut) {
               const uint32_t vn = nkv + 2 * u + 1;
-              const uint8_t* vt = sm + L::kv + (vn % L::stages) * L::tile;
+              const uint8_t* vt = sm + L::kv + (vn % L::stages) * L::kvtile;
               if (ok) ok = mbar_wait_warp(&full[vn % L::stages], (vn / L::stages) & 1, abort_flag);
-              slow = bar_any(1 + x, 128, ok && row_not_finite<T, D>(vt, r));
-              if (slow && ok) sum_visible<T, D>(tm_s, tm_o, vt, first, k0, last, p - P.window, P.sinks);
+              if (ok && !first) ok = mbar_wait_warp(&bars[B_V + x], before, abort_flag);
+              slow = bar_any(1 + x, 128, ok && r < kKeys && row_not_finite<T, D>(vt, r));
+              if (slow && ok) {
+                tc_fence_after();
+                sum_visible<T, D>(tm_s, tm_o, vt, first, k0, last, p - P.window, P.sinks);
+              }
             }
-            if (ok && r == 0) skip_pv[x] = slow;
+            if (ok && r == 0) skip_pv[2 * x + buf] = slow;
             __threadfence_block();
-            __syncwarp();
-            if (ok && lane == 0) {
-              tc_fence_before();
-              mbar_arrive(&bars[B_P + x]);
-            }
           }
           first = false;
           if (ok) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars[B_P + 2 + x]);
+            if (lane == 0) mbar_arrive(&bars[B_P + 2 * x + buf]);
           }
         }
         // -------------------------------------------- o = O / l
@@ -710,14 +738,15 @@ int validate(const gdn_window_attn_args* a) {
   return GDN_OK;
 }
 
-bool make_map(CUtensorMap* m, const gdn_window_attn_args* a, const void* base, const int64_t* st, int rows, int heads) {
+bool make_map(CUtensorMap* m, const gdn_window_attn_args* a, const void* base, const int64_t* st, int rows, int heads,
+              int box_rows) {
   const CUtensorMapDataType dt =
       a->dtype == GDN_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const uint64_t dims[4] = {uint64_t(a->D), uint64_t(rows), uint64_t(heads), uint64_t(a->B)};
   // a dimension of one element may come with any stride: it is never taken
   auto bytes = [&](int64_t s, int n) { return n > 1 ? uint64_t(s) * 2 : uint64_t(a->D) * 2; };
   const uint64_t strides[3] = {bytes(st[1], rows), bytes(st[2], heads), bytes(st[0], a->B)};
-  const uint32_t box[4] = {64, kTile, 1, 1};
+  const uint32_t box[4] = {64, uint32_t(box_rows), 1, 1};
   return make_tmap(m, dt, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
@@ -741,8 +770,8 @@ int run(const gdn_window_attn_args* a, void* stream) {
   if (!device_is_sm100(&dev)) return GDN_ERR_NO_DEVICE;
   Params p;
   memset(&p, 0, sizeof(p));
-  if (!make_map(&p.tm_q, a, a->q, a->q_stride, a->T, a->H) || !make_map(&p.tm_k, a, a->k, a->k_stride, a->S, a->HK) ||
-      !make_map(&p.tm_v, a, a->v, a->v_stride, a->S, a->HK))
+  if (!make_map(&p.tm_q, a, a->q, a->q_stride, a->T, a->H, kTile) || !make_map(&p.tm_k, a, a->k, a->k_stride, a->S, a->HK, kKeys) ||
+      !make_map(&p.tm_v, a, a->v, a->v_stride, a->S, a->HK, kKeys))
     return GDN_ERR_CUDA;
   p.lengths = a->lengths;
   p.o = a->o;
