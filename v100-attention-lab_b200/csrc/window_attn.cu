@@ -16,11 +16,12 @@
 // neighbouring tiles of one head.  So every K/V tile fetched feeds two
 // products, and while one tile's softmax runs the tensor core works on the
 // other's.  One CTA per SM takes item after item; its loads and first scores
-// of the next item run under the last one's epilogue.  Warps: 2 x 4 softmax
-// (one thread per query row), one that fetches K/V tiles by TMA, one that
-// issues the MMAs.  TMEM holds both score tiles and both outputs; the
-// probabilities overwrite their scores' columns and are the second product's
-// TMEM operand, so they never touch shared memory.
+// of the next item run under the last one's epilogue.  Warps: 2 x 8 softmax
+// (two threads per query row, 32 of a tile's 64 keys each), one that fetches
+// tiles by TMA, two that issue the MMAs (one for each query tile: issuing, at 35 cycles
+// an instruction, takes longer than the products).  TMEM holds two score buffers and the
+// output of both query tiles; the probabilities overwrite their scores' columns
+// and are the second product's TMEM operand, so they never touch shared memory.
 //
 // Masks.  Only tiles that some mask cuts are masked element by element.  In
 // those a key hidden from a row has probability 0, and 0 times a value that is
@@ -37,6 +38,7 @@
 
 #include <cstdint>
 #include <cstring>
+#include <type_traits>
 
 namespace gdn {
 namespace wa {
@@ -44,8 +46,13 @@ namespace {
 
 constexpr int kTile = 128;          // query rows per tile
 constexpr int kKeys = 64;           // keys per tile
-constexpr int kTmaWarp = 8, kMmaWarp = 9;
-constexpr int kThreads = 320;
+constexpr int kSoftmaxWarps = 16;   // 8 per query tile: 4 lane quarters x 2 halves of the keys
+constexpr int kTmaWarp = 16, kMmaWarp = 17;  // and kMmaWarp + 1: a query tile's products each
+// Five warpgroups, so that registers can be moved between them: 96 each at
+// launch, then 4 x 104 for the softmax warps and 64 for the others (480 in all).
+constexpr int kThreads = 20 * 32;
+// Named barriers: 1, 2 a query tile's group; 3 all warps; 4 .. 11 the two warps that share rows.
+constexpr int kBarGroup = 1, kBarAll = 3, kBarPair = 4;
 constexpr int kMaxItems = 8192;     // of one CTA
 constexpr uint32_t kTmCols = 512;
 constexpr uint32_t kTmS = 0, kTmO = 256;  // + 128 x tile (+ 64 x buffer of the scores)
@@ -67,11 +74,13 @@ template <int D>
 struct Lay {
   static constexpr uint32_t boxes = D / 64;               // 64-column boxes of a tile
   static constexpr uint32_t qtile = boxes * 16384, kvtile = boxes * 8192;  // bytes
-  static constexpr uint32_t stages = 8;
+  static constexpr uint32_t stages = 4;                   // of the ring; a stage holds V of one key tile and K of the
+  static constexpr uint32_t stage = 2 * kvtile;           // one two on: what the MMA warp takes in one step
   static constexpr uint32_t q = 0;                        // two query tiles
-  static constexpr uint32_t kv = 2 * qtile;               // ring of K and V tiles
-  static constexpr uint32_t out = kv + stages * kvtile;      // [8 warps][32 rows][64 columns] of outputs
-  static constexpr uint32_t bars = out + 32768;
+  static constexpr uint32_t kv = 2 * qtile;
+  static constexpr uint32_t out = kv + stages * stage;    // [16 warps][32 rows][16 columns] of outputs
+  static constexpr uint32_t red = out + 16384;            // [2][2][2][128] row maxima (two in turn), sums
+  static constexpr uint32_t bars = red + 4096;
   static constexpr uint32_t misc = bars + 8 * (2 * stages + 20);
   static constexpr uint32_t redo = misc + 64;             // one bit per item of this CTA
   static constexpr uint32_t bytes = redo + kMaxItems / 8;
@@ -143,25 +152,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 64 columns of this thread's TMEM lane, with the wait in the same statement.
-__device__ __forceinline__ void tmem_ld64w(uint32_t taddr, float* v) {
-  uint32_t r[64];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
-        "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
-        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
-        "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-      : "r"(taddr)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
-}
-
 // Two fp32 operations in one instruction.
 struct F2 {
   uint64_t v;
@@ -187,6 +177,9 @@ __device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
   return r;
 }
 
+template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 template <typename T> struct Pair;
 template <> struct Pair<__half> {
   static __device__ __forceinline__ __half2 zero() { return __floats2half2_rn(0.f, 0.f); }
@@ -204,11 +197,6 @@ struct Rows {
 
   // whether it has a row that sees anything (then its first row sees itself)
   __device__ __forceinline__ bool used() const { return p1 >= p0 && p0 < len; }
-  // whether every row sees every key of the tile at k0
-  __device__ __forceinline__ bool whole(int k0) const {
-    const int k1 = k0 + kKeys - 1;
-    return k1 <= p0 && k1 < len && (k1 < sinks || p1 - k0 < window);
-  }
 };
 
 // The key tiles, by their order in an item, that one query tile sees: some of the
@@ -216,7 +204,6 @@ struct Rows {
 struct Seen {
   int sinks, from, to;
   __device__ __forceinline__ bool operator()(int u) const { return u >= 0 && u <= to && (u < sinks || u >= from); }
-  __device__ __forceinline__ int tiles() const { return to < 0 ? 0 : sinks + (to - from + 1); }
   __device__ __forceinline__ int first() const { return sinks > 0 ? 0 : from; }
   __device__ __forceinline__ int last() const { return to; }
 };
@@ -283,17 +270,19 @@ __device__ __forceinline__ uint32_t tmem_ld1w(uint32_t taddr) {
 
 // O (+)= P V of one key tile over this row's visible keys alone, on the CUDA
 // cores: for tiles whose values are not all finite.  P is read back from TMEM.
+// Each of a row's two threads takes half the columns (tm_o: its first).
 template <typename T, int D>
-__device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uint8_t* vt, bool first, int k0, int last,
-                                         int behind, int sinks) {
-  for (int c0 = 0; c0 < D; c0 += 32) {
+__device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uint8_t* vt, int half, bool first, int k0,
+                                         int last, int behind, int sinks) {
+  for (int c1 = 0; c1 < D / 2; c1 += 32) {
+    const int c0 = half * (D / 2) + c1;
     float o[32];
     uint32_t ou[32];
     if (first) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) o[i] = 0.f;
     } else {
-      tmem_ld32w(tm_o + c0, o);
+      tmem_ld32w(tm_o + c1, o);
     }
     for (int j = 0; j < kKeys; ++j) {
       const float2 pp = Cvt<T>::unpack(tmem_ld1w(tm_p + (j >> 1)));
@@ -320,25 +309,19 @@ __device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uin
     }
 #pragma unroll
     for (int i = 0; i < 32; ++i) ou[i] = __float_as_uint(o[i]);
-    tmem_st32(tm_o + c0, ou);
+    tmem_st32(tm_o + c1, ou);
     tmem_wait_st();
   }
 }
 
-// Masked scores of one tile: this row's visible keys are those up to hi, from lo on or below sk.
+// Masked scores of half a tile: this row's visible keys are those up to hi, from lo on or below sk.
 __device__ __forceinline__ void mask_row(float* s, int hi, int lo, int sk) {
+  // bits of the columns < n
+  auto below = [](int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); };
+  const uint32_t see = below(hi + 1) & (~below(lo) | below(sk));
 #pragma unroll
-  for (int w = 0; w < kKeys / 32; ++w) {
-    // bits of the 32 columns from 32 w on
-    auto below = [&](int n) {  // columns < n
-      n -= 32 * w;
-      return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
-    };
-    const uint32_t see = below(hi + 1) & (~below(lo) | below(sk));
-#pragma unroll
-    for (int c = 0; c < 32; ++c)
-      if (!(see & (1u << c))) s[32 * w + c] = -INFINITY;
-  }
+  for (int c = 0; c < 32; ++c)
+    if (!(see & (1u << c))) s[c] = -INFINITY;
 }
 
 // Whether a value of this thread's key row of the tile is not finite (times 0 it is NaN).
@@ -377,11 +360,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   if (tid == 0) {
     for (uint32_t i = 0; i < L::stages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], 2);  // both query tiles' products
     }
     for (int i = 0; i < B_COUNT; ++i) {
-      const bool softmax = (i >= B_P && i < B_P + 4) || i >= B_OE;  // arrived at by a group's four warps
-      mbar_init(&bars[i], softmax ? 4 : 1);
+      const bool softmax = (i >= B_P && i < B_P + 4) || i >= B_OE;  // arrived at by a group's warps
+      mbar_init(&bars[i], softmax ? kSoftmaxWarps / 2 : 1);
     }
     *abort_flag = 0;
     *any_redo = 0;
@@ -400,17 +383,18 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
 
   // A second, careful pass follows if the first one noted any item; all warps meet in between.
   auto again = [&](bool careful) {
-    named_bar(3, kThreads);
+    named_bar(kBarAll, kThreads);
     return !careful && *any_redo && !*abort_flag;
   };
   // Counts over all items and passes, for the barriers' phases:
-  uint32_t nkv = 0;           // ring slots used
-  uint32_t nq0 = 0, nq1 = 0;  // items that used query tile 0, 1 (softmax: the first for its own)
-  uint32_t ns0 = 0, ns1 = 0;  // key tiles of query tile 0, 1 (the same): scores
-  uint32_t np0 = 0, np1 = 0;  // and products
-  bool ok = true, careful = false;
+  uint32_t nkv = 0;           // ring stages used
+  uint32_t nq0 = 0, nq1 = 0;  // items that used query tile 0, 1 (a role of one tile: the first)
+  uint32_t ns0 = 0, np0 = 0;  // key tiles of the role's query tile: scores, products
+  bool ok = true;
 
-  if (warp >= 8) {
+  if (warp >= kSoftmaxWarps) {
+    regs_less<64>();
+    bool careful = false;
     do {
       if (warp == kTmaWarp) {
         // -------------------------------------------- producer: Q tiles, then K0 V0 K1 V1 ...
@@ -432,139 +416,154 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
             __syncwarp();
             ++nq;
           }
-          for (int n = 0; n < 2 * it.count && ok; ++n) {
+          for (int u = -2; it.count > 0 && u < it.count && ok; ++u) {
             const uint32_t s = nkv % L::stages;
             if (nkv >= L::stages) ok = mbar_wait_warp(&empty[s], (nkv / L::stages - 1) & 1, abort_flag);
             if (!ok) break;
             if (lane == 0) {
-              mbar_arrive_expect_tx(&full[s], L::kvtile);
-              for (uint32_t c = 0; c < L::boxes; ++c)
-                tma_load_4d(sm + L::kv + s * L::kvtile + c * 8192, (n & 1) ? &P.tm_v : &P.tm_k, &full[s], c * 64,
-                            it.key0(n >> 1), it.hk, it.b);
+              uint8_t* dst = sm + L::kv + s * L::stage;
+              const bool v = u >= 0, k = u + 2 < it.count;
+              mbar_arrive_expect_tx(&full[s], (v + k) * L::kvtile);
+              for (uint32_t c = 0; c < L::boxes; ++c) {
+                if (v) tma_load_4d(dst + c * 8192, &P.tm_v, &full[s], c * 64, it.key0(u), it.hk, it.b);
+                if (k) tma_load_4d(dst + L::kvtile + c * 8192, &P.tm_k, &full[s], c * 64, it.key0(u + 2), it.hk, it.b);
+              }
             }
             __syncwarp();
             ++nkv;
           }
         }
-      } else if (warp == kMmaWarp) {
+      } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // -------------------------------------------- MMA issue (the whole warp; elect.sync inside)
         constexpr uint32_t kBf16 = Cvt<T>::kIsBf16;
         constexpr uint32_t id_s = idesc_f16(128, kKeys, kBf16, 0, 0), id_o = idesc_f16(128, D, kBf16, 0, 1);
-        auto wait_kv = [&](uint32_t n) { return mbar_wait_warp(&full[n % L::stages], (n / L::stages) & 1, abort_flag); };
+        const int x = warp - kMmaWarp;
+        const uint32_t tm_s = tmem + kTmS + x * 128, tm_o = tmem + kTmO + x * 128;
+        const uint32_t q_lo = ((sb + L::q + x * L::qtile) >> 4) | (1u << 16);
         for (int j = 0, i = blockIdx.x; i < P.items && ok; ++j, i += gridDim.x) {
           if (careful && !(redo[j >> 5] >> (j & 31) & 1)) continue;
           const Item it = make_item(P, i);
           if (it.count == 0) continue;
-          const Rows rows0 = it.rows(P, 0), rows1 = it.rows(P, 1);
-          const Seen seen0 = it.seen(rows0), seen1 = it.seen(rows1);
-          int left0 = seen0.tiles(), left1 = seen1.tiles();  // products still to be issued
-          const int last0 = seen0.last(), last1 = seen1.last(), first0 = seen0.first(), first1 = seen1.first();
+          const Rows rows = it.rows(P, x);
+          const Seen seen = it.seen(rows);
+          const int first = seen.first(), last = seen.last();
           // Scores run two key tiles ahead of the products, so that a softmax group
           // finds its next tile's ready.
           for (int u = -2; u < it.count && ok; ++u) {
-            const uint32_t vs = (nkv + 2 * u + 1) % L::stages, ks = (nkv + 2 * u + 4) % L::stages;
-            const uint32_t v_lo = ((sb + L::kv + vs * L::kvtile) >> 4) | (512u << 16);  // 8192 bytes between its boxes
-            const uint32_t k_lo = ((sb + L::kv + ks * L::kvtile) >> 4) | (1u << 16);
-            if (u >= 0) ok = wait_kv(nkv + 2 * u + 1);
-            if (ok && u + 2 < it.count) ok = wait_kv(nkv + 2 * u + 4);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const Seen& seen = x ? seen1 : seen0;
-              int& left = x ? left1 : left0;
-              const uint32_t nq = x ? nq1 : nq0;
-              uint32_t &ns = x ? ns1 : ns0, &np = x ? np1 : np0;
-              if (ok && seen(u)) {
-                const bool fresh = u == (x ? first1 : first0);  // this item's first product: O is written, not added to
-                const uint32_t buf = np & 1;
-                ok = mbar_wait_warp(&bars[B_P + 2 * x + buf], (np >> 1) & 1, abort_flag);
-                // the last item's output must have left O
-                if (ok && fresh && nq > 0) ok = mbar_wait_warp(&bars[B_OE + x], (nq - 1) & 1, abort_flag);
-                if (!ok) continue;
-                ++np;
-                tc_fence_after();
-                if (!careful || !skip_pv[2 * x + buf])
-                  mma4_ts(tmem + kTmO + x * 128, tmem + kTmS + x * 128 + buf * 64, v_lo, kDescHi, id_o, !fresh);
-                mma_commit_warp(&bars[B_V + x]);
-                if (--left == 0) mma_commit_warp(&bars[B_O + x]);
-              }
-              // A score buffer is written again two tiles on: in issue order after the
-              // product that read its probabilities.
-              if (ok && seen(u + 2)) {
-                if (u + 2 == (x ? first1 : first0)) ok = mbar_wait_warp(&bars[B_Q + x], nq & 1, abort_flag);
-                if (!ok) continue;
-                const uint32_t q_lo = ((sb + L::q + x * L::qtile) >> 4) | (1u << 16);
-                const uint32_t buf = ns & 1;
-                ++ns;
-#pragma unroll
-                for (uint32_t c = 0; c < L::boxes; ++c)
-                  mma4_ss(tmem + kTmS + x * 128 + buf * 64, q_lo + c * 1024, kDescHi, k_lo + c * 512, kDescHi, id_s, c);
-                mma_commit_warp(&bars[B_S + 2 * x + buf]);
-                if (u + 2 == (x ? last1 : last0)) mma_commit_warp(&bars[B_QE + x]);
-              }
+            const uint32_t s = nkv % L::stages;
+            ok = mbar_wait_warp(&full[s], (nkv / L::stages) & 1, abort_flag);
+            ++nkv;
+            if (ok && seen(u)) {
+              const uint32_t v_lo = ((sb + L::kv + s * L::stage) >> 4) | (512u << 16);  // 8192 bytes between its boxes
+              const bool fresh = u == first;  // this item's first product: O is written, not added to
+              const uint32_t buf = np0 & 1;
+              ok = mbar_wait_warp(&bars[B_P + 2 * x + buf], (np0 >> 1) & 1, abort_flag);
+              // the last item's output must have left O
+              if (ok && fresh && nq0 > 0) ok = mbar_wait_warp(&bars[B_OE + x], (nq0 - 1) & 1, abort_flag);
+              if (!ok) break;
+              ++np0;
+              tc_fence_after();
+              if (!careful || !skip_pv[2 * x + buf]) mma4_ts(tm_o, tm_s + buf * 64, v_lo, kDescHi, id_o, !fresh);
+              mma_commit_warp(&bars[B_V + x]);
+              if (u == last) mma_commit_warp(&bars[B_O + x]);
             }
-            if (ok) {
-              if (u >= 0) mma_commit_warp(&empty[vs]);
-              if (u + 2 < it.count) mma_commit_warp(&empty[ks]);
+            // A score buffer is written again two tiles on: in issue order after the
+            // product that read its probabilities.
+            if (ok && seen(u + 2)) {
+              const uint32_t k_lo = ((sb + L::kv + s * L::stage + L::kvtile) >> 4) | (1u << 16);
+              if (u + 2 == first) ok = mbar_wait_warp(&bars[B_Q + x], nq0 & 1, abort_flag);
+              if (!ok) break;
+              const uint32_t buf = ns0 & 1;
+              ++ns0;
+#pragma unroll
+              for (uint32_t c = 0; c < L::boxes; ++c)
+                mma4_ss(tm_s + buf * 64, q_lo + c * 1024, kDescHi, k_lo + c * 512, kDescHi, id_s, c);
+              mma_commit_warp(&bars[B_S + 2 * x + buf]);
+              if (u + 2 == last) mma_commit_warp(&bars[B_QE + x]);
             }
+            if (ok) mma_commit_warp(&empty[s]);
           }
-          nkv += 2 * it.count;
-          nq0 += rows0.used();
-          nq1 += rows1.used();
+          nq0 += rows.used();
         }
       }
     } while (careful = again(careful), careful);
   } else {
-    // ------------------------------------------------ softmax: thread = one query row of tile x
+    regs_more<104>();
+    // ------------------------------------------------ softmax: two threads per query row of tile x
     // After an abort a warp runs on without waiting or computing, so that the
     // group's barriers still meet.
-    const int x = warp >> 2;
-    const int r = tid & 127;
-    const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t tm_s0 = tmem + lane_base + kTmS + x * 128, tm_o = tmem + lane_base + kTmO + x * 128;
+    const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_base = uint32_t(quarter * 32) << 16;
+    const uint32_t tm_s0 = tmem + lane_base + kTmS + x * 128, tm_o = tmem + lane_base + kTmO + x * 128 + half * (D / 2);
+    const int pair = kBarPair + x * 4 + quarter;
+    float* red = reinterpret_cast<float*>(sm + L::red) + x * 256 + r;  // [turn][x][half][row]
     const float sl2 = P.scale_log2;
-    do {
+    // Two copies of the loop: the careful one's calls would cost the other its registers.
+    auto softmax_pass = [&](auto kind) {
+      constexpr bool careful = decltype(kind)::value;
 #pragma unroll 1
-      for (int j = 0, i = blockIdx.x; i < P.items; ++j, i += gridDim.x) {
+      for (int i = blockIdx.x; i < P.items; i += gridDim.x) {
+        const int j = (i - int(blockIdx.x)) / int(gridDim.x);
         if (careful && !(redo[j >> 5] >> (j & 31) & 1)) continue;
-        const Item it = make_item(P, i);
-        const Rows rows = it.rows(P, x);
-        const bool exists = it.row(P, x) + r < P.T;
-        if (!rows.used()) {
-          if (exists) {
-            T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_t * (long long)(it.row(P, x) + r) + P.so_h * it.head(P, x);
-            for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(op)[c] = make_uint4(0, 0, 0, 0);
+        // What the loop below keeps of the item, in few registers (a spilled one
+        // would come from L2): its key tiles in this tile's own order are n_sink
+        // ones from key 0, then those from key `from` on; those with k0 <= all_to
+        // and either k0 > all_from or k0 + kKeys <= sinks are whole.
+        int tiles, n_sink, from, len, p, all_to, all_from;
+        const uint32_t base = nkv + 2;  // ring stage of the item's first V
+        {
+          const Item it = make_item(P, i);
+          const Rows rows = it.rows(P, x);
+          if (it.count > 0) nkv += it.count + 2;
+          if (!rows.used()) {
+            if (it.row(P, x) + r < P.T) {
+              T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_t * (long long)(it.row(P, x) + r) + P.so_h * it.head(P, x);
+              for (int c = half; c < D / 8; c += 2) reinterpret_cast<uint4*>(op)[c] = make_uint4(0, 0, 0, 0);
+            }
+            continue;
           }
-          nkv += 2 * it.count;
-          continue;
+          const Seen seen = it.seen(rows);
+          n_sink = seen.sinks;
+          from = it.key0(seen.from);
+          tiles = n_sink + seen.to - seen.from + 1;
+          len = it.len;
+          p = rows.p0 + r;
+          all_to = (rows.p0 < len - 1 ? rows.p0 : len - 1) - (kKeys - 1);
+          all_from = rows.p1 - P.window;
         }
-        const Seen seen = it.seen(rows);
-        const int p = rows.p0 + r;
-        const int last = p < it.len ? p : -1;  // the last visible key; rows behind the sequence see none
-        float m = -INFINITY, l = 0.f;          // running reference maximum (raw scores) and sum
-        bool first = true;
+        float m = -INFINITY, l = 0.f;  // running reference maximum (raw scores); sum over this half
 #pragma unroll 1
-        for (int u = 0; u < it.count; ++u) {
-          if (!seen(u)) continue;
-          const int k0 = it.key0(u);
-          const bool cut = !rows.whole(k0);
+        for (int t = 0; t < tiles; ++t) {
+          const int k0 = t < n_sink ? t * kKeys : from + (t - n_sink) * kKeys;
+          const bool cut = k0 > all_to || (k0 <= all_from && k0 + kKeys > P.sinks);
           const uint32_t buf = ns0 & 1, before = (ns0 - 1) & 1;
           const uint32_t tm_s = tm_s0 + buf * 64;
           if (ok) ok = mbar_wait_warp(&bars[B_S + 2 * x + buf], (ns0 >> 1) & 1, abort_flag);
-          ++ns0;
+          float s[32];
+          float mt = 0.f;
           if (ok) {
             tc_fence_after();
-            float s[kKeys];
-            tmem_ld64w(tm_s, s);
-            if (cut) mask_row(s, last - k0, p - P.window + 1 - k0, P.sinks - k0);
-            float mx[8];
+            tmem_ld32w(tm_s + 32 * half, s);
+            if (cut) {
+              const int c0 = k0 + 32 * half;
+              mask_row(s, (p < len ? p : -1) - c0, p - P.window + 1 - c0, P.sinks - c0);  // rows behind the sequence see none
+            }
+            float mx[4];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) mx[c] = fmaxf(s[c], s[c + 8]);
+            for (int c = 0; c < 4; ++c) mx[c] = fmaxf(s[c], s[c + 4]);
 #pragma unroll
-            for (int c = 16; c < kKeys; c += 16)
+            for (int c = 8; c < 32; c += 8)
 #pragma unroll
-              for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], fmaxf(s[c + e], s[c + 8 + e]));
-            const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                                   fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+              for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(s[c + e], s[c + 4 + e]));
+            mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            red[buf * 512 + half * 128] = mt;
+          }
+          // Both halves have their scores and know each other's maximum from here on.
+          named_bar(pair, 64);
+          ++ns0;
+          if (ok) {
+            mt = fmaxf(mt, red[buf * 512 + (half ^ 1) * 128]);
             // The reference follows the maximum only when a probability would
             // pass 2^8: most tiles then leave O as it is.
             const bool up = (mt - m) * sl2 > 8.f || (m == -INFINITY && mt > m);
@@ -572,19 +571,19 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
               const float corr = !up ? 1.f : (m == -INFINITY ? 0.f : fast_exp2((m - mt) * sl2));
               if (up) m = mt;
               l *= corr;
-              if (!first) {
+              if (t > 0) {
                 // the product before has to be in O
                 ok = mbar_wait_warp(&bars[B_V + x], before, abort_flag);
                 if (ok) {
                   tc_fence_after();
 #pragma unroll 1
-                  for (int c = 0; c < D; c += 32) {
-                    float o[32];
-                    tmem_ld32w(tm_o + c, o);
-                    uint32_t ou[32];
+                  for (int c = 0; c < D / 2; c += 16) {
+                    float o[16];
+                    tmem_ld16w(tm_o + c, o);
+                    uint32_t ou[16];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) ou[e] = __float_as_uint(o[e] * corr);
-                    tmem_st32(tm_o + c, ou);
+                    for (int e = 0; e < 16; ++e) ou[e] = __float_as_uint(o[e] * corr);
+                    tmem_st16(tm_o + c, ou);
                   }
                 }
               }
@@ -592,21 +591,18 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
             const float ms = m == -INFINITY ? 0.f : m * sl2;
             const F2 sl = f2(sl2, sl2), nm = f2(-ms, -ms);
             F2 sum0 = f2(0.f, 0.f), sum1 = sum0;
+            uint32_t pk[16];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int c = 0; c < 16; ++c) {
-                float2 e = f2_get(f2_fma(f2(s[32 * h + 2 * c], s[32 * h + 2 * c + 1]), sl, nm));
-                e = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-                if (c & 1)
-                  sum1 = f2_add(sum1, f2(e.x, e.y));
-                else
-                  sum0 = f2_add(sum0, f2(e.x, e.y));
-                pk[c] = Cvt<T>::pack(e.x, e.y);
-              }
-              tmem_st16(tm_s + 16 * h, pk);
+            for (int c = 0; c < 16; ++c) {
+              float2 e = f2_get(f2_fma(f2(s[2 * c], s[2 * c + 1]), sl, nm));
+              e = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+              if (c & 1)
+                sum1 = f2_add(sum1, f2(e.x, e.y));
+              else
+                sum0 = f2_add(sum0, f2(e.x, e.y));
+              pk[c] = Cvt<T>::pack(e.x, e.y);
             }
+            tmem_st16(tm_s + 16 * half, pk);
             const float2 sum = f2_get(f2_add(sum0, sum1));
             l += sum.x + sum.y;
             tmem_wait_st();
@@ -614,20 +610,22 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           if (careful) {
             bool slow = false;
             if (cut) {
-              const uint32_t vn = nkv + 2 * u + 1;
-              const uint8_t* vt = sm + L::kv + (vn % L::stages) * L::kvtile;
-              if (ok) ok = mbar_wait_warp(&full[vn % L::stages], (vn / L::stages) & 1, abort_flag);
-              if (ok && !first) ok = mbar_wait_warp(&bars[B_V + x], before, abort_flag);
-              slow = bar_any(1 + x, 128, ok && r < kKeys && row_not_finite<T, D>(vt, r));
+              const Item it = make_item(P, i);
+              const uint32_t n = base + (t < n_sink ? t : it.seen(it.rows(P, x)).from + (t - n_sink));
+              const uint8_t* vt = sm + L::kv + n % L::stages * L::stage;
+              if (ok) ok = mbar_wait_warp(&full[n % L::stages], (n / L::stages) & 1, abort_flag);
+              if (ok && t > 0) ok = mbar_wait_warp(&bars[B_V + x], before, abort_flag);
+              tc_fence_before();
+              // (the barrier is also where both halves' probabilities meet)
+              slow = bar_any(kBarGroup + x, 256, ok && half == 0 && r < kKeys && row_not_finite<T, D>(vt, r));
               if (slow && ok) {
                 tc_fence_after();
-                sum_visible<T, D>(tm_s, tm_o, vt, first, k0, last, p - P.window, P.sinks);
+                sum_visible<T, D>(tm_s, tm_o, vt, half, t == 0, k0, p < len ? p : -1, p - P.window, P.sinks);
               }
             }
-            if (ok && r == 0) skip_pv[2 * x + buf] = slow;
+            if (ok && half == 0 && r == 0) skip_pv[2 * x + buf] = slow;
             __threadfence_block();
           }
-          first = false;
           if (ok) {
             tc_fence_before();
             __syncwarp();
@@ -636,26 +634,31 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
         }
         // -------------------------------------------- o = O / l
         if (ok) ok = mbar_wait_warp(&bars[B_O + x], nq0 & 1, abort_flag);
+        red[(ns0 & 1) * 512 + half * 128] = l;
+        named_bar(pair, 64);
+        l += red[(ns0 & 1) * 512 + (half ^ 1) * 128];
+        named_bar(pair, 64);  // read before the next item's maxima
         if (ok) {
           tc_fence_after();
-          const bool live = last >= 0;
+          const Item it = make_item(P, i);
+          const bool live = p < len;
           const float inv = 1.f / l;
           float odd = 0.f;  // NaN if some output is not finite
-          // Rows leave through shared memory, so that a store covers whole lines.
-          uint8_t* stage = sm + L::out + warp * 4096;
-          const int row = it.row(P, x) + (r - lane);  // this warp's first
-          T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_h * it.head(P, x) + P.so_t * (long long)row;
+          // Rows leave through shared memory, so that a store covers whole sectors.
+          uint8_t* stage = sm + L::out + warp * 1024;
+          const int row = it.row(P, x) + quarter * 32;  // this warp's first
+          T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_h * it.head(P, x) + P.so_t * (long long)row + half * (D / 2);
 #pragma unroll 1
-          for (int half = 0; half < D / 64; ++half) {
-            float o[64];
-            tmem_ld64w(tm_o + 64 * half, o);
-            if (half == D / 64 - 1) {
+          for (int part = 0; part < D / 32; ++part) {
+            float o[16];
+            tmem_ld16w(tm_o + 16 * part, o);
+            if (part == D / 32 - 1) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&bars[B_OE + x]);
             }
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
+            for (int c = 0; c < 2; ++c) {
               uint4 w;
               uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
@@ -665,26 +668,31 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
                 odd = fmaf(b2, 0.f, odd);
                 wp[e] = live ? Cvt<T>::pack(a, b2) : 0u;
               }
-              *reinterpret_cast<uint4*>(stage + sw128_off(lane, c)) = w;
+              // rows of 32 bytes, their two pieces swapped every fourth row
+              *reinterpret_cast<uint4*>(stage + lane * 32 + ((c ^ ((lane >> 2) & 1)) << 4)) = w;
             }
             __syncwarp();
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const int rr = 4 * c + (lane >> 3);
-              const uint4 w = *reinterpret_cast<const uint4*>(stage + sw128_off(rr, lane & 7));
-              if (row + rr < P.T) reinterpret_cast<uint4*>(op + P.so_t * (long long)rr + 64 * half)[lane & 7] = w;
+            for (int c = 0; c < 2; ++c) {
+              const int rr = 16 * c + (lane >> 1);
+              const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 32 + (((lane & 1) ^ ((rr >> 2) & 1)) << 4));
+              if (row + rr < P.T) reinterpret_cast<uint4*>(op + P.so_t * (long long)rr + 16 * part)[lane & 1] = w;
             }
             __syncwarp();
           }
-          if (!careful && exists && live && odd != odd) {
+          if (!careful && row + lane < P.T && live && odd != odd) {
             atomicOr(&redo[j >> 5], 1u << (j & 31));
             *any_redo = 1;
           }
         }
         ++nq0;
-        nkv += 2 * it.count;
       }
-    } while (careful = again(careful), careful);
+    };
+    softmax_pass(std::false_type{});
+    if (again(false)) {
+      softmax_pass(std::true_type{});
+      again(true);
+    }
   }
   // On an abort the loads and products still in flight end before the CTA leaves.
   if (warp == kTmaWarp && *abort_flag) {
@@ -694,21 +702,22 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     for (uint32_t n = nkv > L::stages ? nkv - L::stages : 0; n < nkv; ++n)
       mbar_wait(&full[n % L::stages], (n / L::stages) & 1, &never);
   }
+  if ((warp == kMmaWarp || warp == kMmaWarp + 1) && *abort_flag) {
+    // a commit of its own: every product this warp has issued has ended when it arrives
+    uint64_t* done = &bars[B_COUNT + warp - kMmaWarp];
+    if (lane == 0) {
+      mbar_init(done, 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+    mma_commit_warp(done);
+    volatile int never = 0;
+    mbar_wait(done, 0, &never);
+    __syncwarp();
+  }
   __syncthreads();
   if (tid == 0 && *abort_flag && P.status) atomicOr(P.status, 1 << GDN_ERR_TIMEOUT);
   if (warp == kMmaWarp) {
-    if (*abort_flag) {
-      // a commit of its own: every product issued so far has ended when it arrives
-      if (lane == 0) {
-        mbar_init(&bars[B_COUNT], 1);
-        fence_mbar_init();
-      }
-      __syncwarp();
-      mma_commit_warp(&bars[B_COUNT]);
-      volatile int never = 0;
-      mbar_wait(&bars[B_COUNT], 0, &never);
-      __syncwarp();
-    }
     tc_fence_after();
     tmem_dealloc(tmem, kTmCols);
   }
