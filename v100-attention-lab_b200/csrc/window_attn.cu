@@ -53,6 +53,7 @@ constexpr int kTmaWarp = 16, kMmaWarp = 17;  // and kMmaWarp + 1: a query tile's
 constexpr int kThreads = 20 * 32;
 // Named barriers: 1, 2 a query tile's group; 3 all warps; 4 .. 11 the two warps that share rows.
 constexpr int kBarGroup = 1, kBarAll = 3, kBarPair = 4;
+constexpr int kPolyPairs = 4;       // of a thread's 16 pairs of exponentials: on the FMA pipe (none: 953 us, 4: 887, 8: 966)
 constexpr int kMaxItems = 8192;     // of one CTA
 constexpr uint32_t kTmCols = 512;
 constexpr uint32_t kTmS = 0, kTmO = 256;  // + 128 x tile (+ 64 x buffer of the scores)
@@ -174,6 +175,36 @@ __device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
 __device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
   F2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+// 2^x on the FMA pipe, for the share of the exponentials that the special-function
+// pipe (16 per clock and SM) has no time for.  Cody-Waite: x = n + r with
+// |r| <= 1/2 by adding and subtracting 1.5 2^23, a polynomial of degree 4 for 2^r
+// (fitted for the least relative error, 2.6e-6, far below the 16-bit rounding
+// that follows), and n added to the exponent.  x <= 127; below -126, and for a
+// hidden key's -infinity, exactly 0: its value may be anything.
+__device__ __forceinline__ float2 exp2_poly(F2 x) {
+  float2 c = f2_get(x);
+  c.x = fmaxf(c.x, -126.f);
+  c.y = fmaxf(c.y, -126.f);
+  const F2 m = f2(c.x, c.y);
+  const F2 z = f2_add(m, f2(12582912.f, 12582912.f));
+  const F2 n = f2_add(z, f2(-12582912.f, -12582912.f));
+  const F2 r = f2_fma(n, f2(-1.f, -1.f), m);
+  F2 y = f2_fma(f2(0.00957016088f, 0.00957016088f), r, f2(0.0559178293f, 0.0559178293f));
+  y = f2_fma(y, r, f2(0.240247428f, 0.240247428f));
+  y = f2_fma(y, r, f2(0.693121791f, 0.693121791f));
+  y = f2_fma(y, r, f2(0.999999285f, 0.999999285f));
+  const float2 yy = f2_get(y), zz = f2_get(z);
+  return make_float2(c.x > -126.f ? __uint_as_float(__float_as_uint(yy.x) + (__float_as_uint(zz.x) << 23)) : 0.f,
+                     c.y > -126.f ? __uint_as_float(__float_as_uint(yy.y) + (__float_as_uint(zz.y) << 23)) : 0.f);
+}
+
+// The larger of three; NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -549,27 +580,31 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
               const int c0 = k0 + 32 * half;
               mask_row(s, (p < len ? p : -1) - c0, p - P.window + 1 - c0, P.sinks - c0);  // rows behind the sequence see none
             }
+            // a NaN among the scores becomes the maximum, and so the row's output
             float mx[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = fmaxf(s[c], s[c + 4]);
+            for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[4 + e], s[8 + e]);
 #pragma unroll
-            for (int c = 8; c < 32; c += 8)
+            for (int c = 12; c < 28; c += 8)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(s[c + e], s[c + 4 + e]));
-            mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+              for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[28 + e], s[28 + e]);
+            mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
             red[buf * 512 + half * 128] = mt;
           }
           // Both halves have their scores and know each other's maximum from here on.
           named_bar(pair, 64);
           ++ns0;
           if (ok) {
-            mt = fmaxf(mt, red[buf * 512 + (half ^ 1) * 128]);
+            const float mo = red[buf * 512 + (half ^ 1) * 128];
+            mt = max3(mt, mo, mo);
             // The reference follows the maximum only when a probability would
             // pass 2^8: most tiles then leave O as it is.
-            const bool up = (mt - m) * sl2 > 8.f || (m == -INFINITY && mt > m);
+            const bool up = !((mt - m) * sl2 <= 8.f) && mt != -INFINITY;
             if (__any_sync(0xffffffffu, up)) {
               const float corr = !up ? 1.f : (m == -INFINITY ? 0.f : fast_exp2((m - mt) * sl2));
-              if (up) m = mt;
+              if (up) m = mt == INFINITY ? NAN : mt;  // infinity less infinity
               l *= corr;
               if (t > 0) {
                 // the product before has to be in O
@@ -595,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
               float2 e = f2_get(f2_fma(f2(s[2 * c], s[2 * c + 1]), sl, nm));
-              e = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+              e = c < kPolyPairs ? exp2_poly(f2(e.x, e.y)) : make_float2(fast_exp2(e.x), fast_exp2(e.y));
               if (c & 1)
                 sum1 = f2_add(sum1, f2(e.x, e.y));
               else
