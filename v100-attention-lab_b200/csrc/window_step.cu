@@ -38,7 +38,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCluster = 8;
 
@@ -56,22 +56,36 @@ struct Params {
   float scale_log2;
 };
 
-template <typename T>
+// One 16 x 8 x 16 step.  With 8 query rows the lower half of A and of the result
+// is zero and takes no registers.
+template <typename T, int HR>
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  if constexpr (Cvt<T>::kIsBf16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if constexpr (HR == 2) {
+    if constexpr (Cvt<T>::kIsBf16)
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                   : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                   : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    float d2, d3;
+    if constexpr (Cvt<T>::kIsBf16)
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
+                   : "+f"(c[0]), "+f"(c[1]), "=f"(d2), "=f"(d3)
+                   : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+    else
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
+                   : "+f"(c[0]), "+f"(c[1]), "=f"(d2), "=f"(d3)
+                   : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+  }
 }
 
 // ROWS query rows (8 or 16) per group; with 8 the lower half of each tile is zero.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kThreads, ROWS == 8 ? 2 : 1) window_step_kernel(const Params P) {
+__global__ void __launch_bounds__(kThreads, 2) window_step_kernel(const Params P) {
   constexpr int KC = D / 32;   // 16-byte pieces of a key per lane
   constexpr int VH = D / 64;   // column halves of V
   constexpr int HR = ROWS / 8;
@@ -121,72 +135,106 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 2 : 1) window_step_kerne
       qf[r][c] = g + 8 * r < rows ? *reinterpret_cast<const uint4*>(qp + P.qs[1] * (g + 8 * r) + c * 32 + t * 8)
                                   : make_uint4(0, 0, 0, 0);
 
-  float acc[VH][8][4];
+  constexpr int NC = 2 * HR;  // accumulators of a lane per 8 columns
+  float acc[VH][8][NC];
 #pragma unroll
-  for (int i = 0; i < VH * 8 * 4; ++i) (&acc[0][0][0])[i] = 0.f;
+  for (int i = 0; i < VH * 8 * NC; ++i) (&acc[0][0][0])[i] = 0.f;
   float m[HR], l[HR];
 #pragma unroll
   for (int r = 0; r < HR; ++r) m[r] = -INFINITY, l[r] = 0.f;
 
   const int ntile = (n + 15) / 16;
-  const int per = (ntile + C * kWarps - 1) / (C * kWarps);
-  const int first = (rank * kWarps + warp) * per;
-  const int end = first + per < ntile ? first + per : ntile;
-  for (int tile = first; tile < end; ++tile) {
+  // A CTA's tiles are a run, dealt out to its warps one by one: what is read at
+  // a time lies close together.
+  const int per = (ntile + C - 1) / C;
+  const int first = rank * per + warp;
+  const int end = rank * per + per < ntile ? rank * per + per : ntile;
+  // A lane's pieces of a tile: keys g and 8 + g of K, keys 2t, 2t+1, 2t+8, 2t+9 of V.
+  uint4 kf[2][KC], vf[4][VH];
+  // Most tiles are 16 slots in a row, old keys all: one address and constant steps.
+  auto run_of = [&](int tile) {
     const int i0 = tile * 16;
-    uint4 kf[2][KC], vf[4][VH];
+    return i0 >= n_sink && i0 + 16 < n && slot_of(i0) + 16 <= P.cap;
+  };
+  auto load_k = [&](int tile) {
+    const int i0 = tile * 16;
+    if (run_of(tile)) {
+      const T* src = kc + P.kcs[1] * (long long)(slot_of(i0) + g) + t * 8;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) kf[j][c] = __ldcs(reinterpret_cast<const uint4*>(src + j * 8 * P.kcs[1] + c * 32));
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int i = i0 + j * 8 + g;
-      const bool isnew = i == n - 1;
-      const T* src = isnew ? kn : kc + P.kcs[1] * (long long)slot_of(i < n ? i : 0);
+      const T* src = i == n - 1 ? kn : kc + P.kcs[1] * (long long)slot_of(i < n ? i : 0);
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         kf[j][c] = make_uint4(0, 0, 0, 0);
         if (i < n) kf[j][c] = *reinterpret_cast<const uint4*>(src + c * 32 + t * 8);
       }
+      // the new key goes into the cache: the lanes that read it write it
+      if (i == n - 1 && grp == 0)
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+          *reinterpret_cast<uint4*>(const_cast<T*>(kc) + P.kcs[1] * (long long)slot_of(i) + c * 32 + t * 8) = kf[j][c];
+    }
+  };
+  auto load_v = [&](int tile) {
+    const int i0 = tile * 16;
+    if (run_of(tile)) {
+      const T* src = vc + P.vcs[1] * (long long)(slot_of(i0) + 2 * t) + g * 8;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < VH; ++c)
+          vf[j][c] = __ldcs(reinterpret_cast<const uint4*>(src + ((j & 1) + (j >> 1) * 8) * P.vcs[1] + c * 64));
+      return;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // keys 2t, 2t+1, 2t+8, 2t+9; zero where there is none
+    for (int j = 0; j < 4; ++j) {  // zero where there is no key
       const int i = i0 + 2 * t + (j & 1) + (j >> 1) * 8;
-      const bool isnew = i == n - 1;
-      const T* src = isnew ? vn : vc + P.vcs[1] * (long long)slot_of(i < n ? i : 0);
+      const T* src = i == n - 1 ? vn : vc + P.vcs[1] * (long long)slot_of(i < n ? i : 0);
 #pragma unroll
       for (int c = 0; c < VH; ++c) {
         vf[j][c] = make_uint4(0, 0, 0, 0);
         if (i < n) vf[j][c] = *reinterpret_cast<const uint4*>(src + c * 64 + g * 8);
       }
+      if (i == n - 1 && grp == 0)
+#pragma unroll
+        for (int c = 0; c < VH; ++c)
+          *reinterpret_cast<uint4*>(const_cast<T*>(vc) + P.vcs[1] * (long long)slot_of(i) + c * 64 + g * 8) = vf[j][c];
     }
-    float s[2][4];
+  };
+  if (first < end) {
+    load_k(first);
+    load_v(first);
+  }
+#pragma unroll 1
+  for (int tile = first; tile < end; tile += kWarps) {
+    const int i0 = tile * 16;
+    float s[2][NC];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+      for (int e = 0; e < NC; ++e) s[j][e] = 0.f;
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         const uint4 a = qf[0][c], a8 = HR == 2 ? qf[HR - 1][c] : make_uint4(0, 0, 0, 0);
-        mma16816<T>(s[j], a.x, a8.x, a.y, a8.y, kf[j][c].x, kf[j][c].y);
-        mma16816<T>(s[j], a.z, a8.z, a.w, a8.w, kf[j][c].z, kf[j][c].w);
+        mma16816<T, HR>(s[j], a.x, a8.x, a.y, a8.y, kf[j][c].x, kf[j][c].y);
+        mma16816<T, HR>(s[j], a.z, a8.z, a.w, a8.w, kf[j][c].z, kf[j][c].w);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (i0 + j * 8 + 2 * t + e >= n) s[j][e] = s[j][2 + e] = -INFINITY;
+        if (i0 + j * 8 + 2 * t + e >= n)
+#pragma unroll
+          for (int r = 0; r < HR; ++r) s[j][2 * r + e] = -INFINITY;
     }
-    // the new key and value go into the cache; lanes that read them write them
-    if (grp == 0 && i0 + 16 >= n && i0 < n) {
-      const int slot = slot_of(n - 1);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (i0 + j * 8 + g == n - 1)
-#pragma unroll
-          for (int c = 0; c < KC; ++c)
-            *reinterpret_cast<uint4*>(const_cast<T*>(kc) + P.kcs[1] * (long long)slot + c * 32 + t * 8) = kf[j][c];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i0 + 2 * t + (j & 1) + (j >> 1) * 8 == n - 1)
-#pragma unroll
-          for (int c = 0; c < VH; ++c)
-            *reinterpret_cast<uint4*>(const_cast<T*>(vc) + P.vcs[1] * (long long)slot + c * 64 + g * 8) = vf[j][c];
-    }
+    // the next tile's keys are fetched under this one's softmax, its values
+    // under the next one's scores: into the registers just used
+    if (tile + kWarps < end) load_k(tile + kWarps);
     uint32_t ph[2][HR], pl[2][HR];  // probabilities of keys (2t, 2t+1) of each half tile, high and low terms
 #pragma unroll
     for (int r = 0; r < HR; ++r) {
@@ -200,8 +248,8 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 2 : 1) window_step_kerne
       l[r] *= corr;
 #pragma unroll
       for (int i = 0; i < VH * 8; ++i) {
-        (&acc[0][0][0])[4 * i + 2 * r] *= corr;
-        (&acc[0][0][0])[4 * i + 2 * r + 1] *= corr;
+        (&acc[0][0][0])[NC * i + 2 * r] *= corr;
+        (&acc[0][0][0])[NC * i + 2 * r + 1] *= corr;
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -223,10 +271,11 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 2 : 1) window_step_kerne
           const uint32_t b0 = __byte_perm(v0, v1, odd ? 0x7632 : 0x5410);
           const uint32_t b1 = __byte_perm(v2, v3, odd ? 0x7632 : 0x5410);
           float* a = acc[c][2 * w + odd];
-          mma16816<T>(a, ph[0][0], HR == 2 ? ph[0][HR - 1] : 0u, ph[1][0], HR == 2 ? ph[1][HR - 1] : 0u, b0, b1);
-          mma16816<T>(a, pl[0][0], HR == 2 ? pl[0][HR - 1] : 0u, pl[1][0], HR == 2 ? pl[1][HR - 1] : 0u, b0, b1);
+          mma16816<T, HR>(a, ph[0][0], HR == 2 ? ph[0][HR - 1] : 0u, ph[1][0], HR == 2 ? ph[1][HR - 1] : 0u, b0, b1);
+          mma16816<T, HR>(a, pl[0][0], HR == 2 ? pl[0][HR - 1] : 0u, pl[1][0], HR == 2 ? pl[1][HR - 1] : 0u, b0, b1);
         }
       }
+    if (tile + kWarps < end) load_v(tile + kWarps);
   }
 
   // ---------------------------------------------- join the warps, then the CTAs
@@ -335,15 +384,15 @@ int launch(const Params& p, int C, dim3 grid, cudaStream_t s, int dev) {
 }
 
 template <typename T, int D>
-int launch_rows(const Params& p, int B, cudaStream_t s, int dev) {
+int launch_rows(const Params& p, int B, int sms, cudaStream_t s, int dev) {
   const int rows = p.G <= 8 ? 8 : 16;
   const int groups = p.HK * ((p.G + rows - 1) / rows);
-  // CTAs along the keys: as many as give every SM two, while each of their
-  // warps still has a tile.
-  const long long own = (long long)B * groups;
+  // CTAs along the keys: the fewest that fill the SMs' last wave to nine
+  // tenths (joining more costs), while each of their warps still has two tiles.
+  const long long own = (long long)B * groups, slots = 2LL * sms;
   const int tiles = (p.window + p.sinks + 15) / 16;
   int C = 1;
-  while (C < kMaxCluster && own * C < 296 && C * kWarps < tiles) C *= 2;
+  while (C < kMaxCluster && C * kWarps * 4 <= tiles && own * C * 10 < (own * C + slots - 1) / slots * slots * 9) C *= 2;
   const dim3 grid(C, groups, B);
   return rows == 8 ? launch<T, D, 8>(p, C, grid, s, dev) : launch<T, D, 16>(p, C, grid, s, dev);
 }
@@ -362,11 +411,13 @@ int run(const gdn_window_step_args* a, void* stream) {
   p.G = a->H / a->HK, p.HK = a->HK;
   p.cap = a->capacity, p.window = a->window, p.sinks = a->sinks;
   p.scale_log2 = a->scale * 1.4426950408889634f;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return cuda_failed();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = a->dtype == GDN_DTYPE_BF16;
   if (a->D == 128)
-    return bf ? launch_rows<__nv_bfloat16, 128>(p, a->B, s, dev) : launch_rows<__half, 128>(p, a->B, s, dev);
-  return bf ? launch_rows<__nv_bfloat16, 64>(p, a->B, s, dev) : launch_rows<__half, 64>(p, a->B, s, dev);
+    return bf ? launch_rows<__nv_bfloat16, 128>(p, a->B, sms, s, dev) : launch_rows<__half, 128>(p, a->B, sms, s, dev);
+  return bf ? launch_rows<__nv_bfloat16, 64>(p, a->B, sms, s, dev) : launch_rows<__half, 64>(p, a->B, sms, s, dev);
 }
 
 }  // namespace
