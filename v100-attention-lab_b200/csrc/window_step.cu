@@ -387,12 +387,14 @@ template <typename T, int D>
 int launch_rows(const Params& p, int B, int sms, cudaStream_t s, int dev) {
   const int rows = p.G <= 8 ? 8 : 16;
   const int groups = p.HK * ((p.G + rows - 1) / rows);
-  // CTAs along the keys: the fewest that fill the SMs' last wave to nine
-  // tenths (joining more costs), while each of their warps still has two tiles.
-  const long long own = (long long)B * groups, slots = 2LL * sms;
+  // CTAs along the keys: as many as still run at once, two on an SM, each warp
+  // with a tile.  A second wave for the sake of a fuller last one does not pay,
+  // joining costs more: 64 sequences, 8 key heads, 4100 keys take 206 us with
+  // one CTA each, 215 with two, 233 with four; 16 with 2052 keys 49, 32 (two), 38.
+  const long long own = (long long)B * groups;
   const int tiles = (p.window + p.sinks + 15) / 16;
-  int C = 1;
-  while (C < kMaxCluster && C * kWarps * 4 <= tiles && own * C * 10 < (own * C + slots - 1) / slots * slots * 9) C *= 2;
+  int C = kMaxCluster;
+  while (C > 1 && (own * C > 2LL * sms || (C - 1) * kWarps >= tiles)) --C;
   const dim3 grid(C, groups, B);
   return rows == 8 ? launch<T, D, 8>(p, C, grid, s, dev) : launch<T, D, 16>(p, C, grid, s, dev);
 }
