@@ -355,14 +355,15 @@ def gdn_step(q, k, v, beta, g, state, *, scale=None, output_dtype=None, use_qk_l
     flags = _prep_flags(use_qk_l2norm_in_kernel, beta_activation, g_activation)
     if g is None and g_activation is not None:
         raise ValueError("g_activation needs a g tensor")
-    for name, t in (("q", q), ("k", k), ("v", v), ("beta", beta), ("g", g), ("state", state)):
-        if t is not None:
-            _check_device(name, t, dev, "q")
+    if not q.is_cuda:
+        raise ValueError(f"q must be a CUDA tensor (got device {dev})")
+    if k.device != dev or v.device != dev or beta.device != dev or state.device != dev or (g is not None and g.device != dev):
+        raise ValueError(f"q, k, v, beta, g and state must be on one device (q is on {dev})")
     if beta.dtype != torch.float32:
         beta = beta.float()
     if g is not None and g.dtype != torch.float32:
         g = g.float()
-    o = torch.empty((B, H, V), dtype=out_dtype, device=dev)
+    o = _empty(v, out_dtype)
     sb, sg, so = beta.stride(), (0, 0) if g is None else g.stride(), o.stride()
     args = _lib.STEP_ARGS.pack(
         _lib.ABI_VERSION, B, H, K, V, _DTYPES[dtype], _DTYPES[out_dtype], flags, 1.0 if scale is None else float(scale), 0,
@@ -409,10 +410,17 @@ def _check_device(name, t, dev, first):
         raise ValueError(f"{name} is on {t.device}, {first} is on {dev}")
 
 
+def _empty(like, dtype):
+    """Uninitialised contiguous tensor of ``like``'s shape and device (empty_like is twice as fast as empty)."""
+    if dtype == like.dtype:
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _launch(fn, where: str, args: bytes, dev: torch.device):
     """Call a C entry point with a packed argument struct on ``dev``'s current stream; raise on its status."""
     idx = dev.index
-    if idx == torch.cuda.current_device():
+    if idx == torch._C._cuda_getDevice():  # current_device() without its check that CUDA is up: a tensor is there
         rc = fn(args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _check_device, _launch, _status_ptr
+from .ops import _DTYPES, _check_device, _empty, _launch, _status_ptr
 
 __all__ = ["gated_scan", "gated_scan_step"]
 
@@ -75,7 +75,7 @@ def _pack(x, g, o_dtype, flags, h0=None, o=None, ht=None, states=None, d_o=None,
 def _forward(x, g, h0, flags, out_dtype, want_ht, want_states):
     lib = _lib.load()
     dev, shape = x.device, x.shape
-    o = torch.empty(shape, dtype=out_dtype, device=dev)
+    o = _empty(x, out_dtype)
     ht = torch.empty((shape[0], shape[2], shape[3]), dtype=torch.float32, device=dev) if want_ht else None
     states = None
     if want_states:
@@ -107,8 +107,7 @@ def _backward(ctx, d_o, dht):
         return None, None, None, None, None, None
     x, g, states = ctx.saved_tensors
     dev = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dg = torch.empty(x.shape, dtype=g.dtype, device=dev)
+    dx, dg = _empty(x, x.dtype), _empty(x, g.dtype)
     need_x, need_g, need_h0 = ctx.needs_input_grad[:3]
     dh0 = torch.empty((x.shape[0],) + x.shape[2:], dtype=torch.float32, device=dev) if need_h0 else None
     if d_o is not None and d_o.stride(-1) != 1:  # e.g. the expanded gradient of a sum
@@ -174,7 +173,12 @@ def gated_scan_step(x, g, state, *, g_activation=None, output_dtype=None):
         raise NotImplementedError("gated_scan_step has no backward: use gated_scan, or torch.no_grad()")
     if g.dtype != torch.float32 and g.dtype != x.dtype:
         g = g.float()
-    o = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    _launch(_lib.load().gdn_gated_scan_fwd_sm100, "gdn_gated_scan_fwd_sm100",
-            _pack(x, g, out_dtype, flags, h0=state, o=o, ht=state), x.device)
+    o = _empty(x, out_dtype)
+    B, H, D = x.shape
+    sx, sg, at = x.stride(), g.stride(), state.data_ptr()
+    args = _lib.GATED_SCAN_ARGS.pack(
+        _lib.ABI_VERSION, B, 1, H, D, _DTYPES[x.dtype], _DTYPES[g.dtype], _DTYPES[out_dtype], flags, 0,
+        x.data_ptr(), sx[0], 0, sx[1], g.data_ptr(), sg[0], 0, sg[1], at, o.data_ptr(), H * D, 0, D, at, 0,
+        0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    _launch(_lib.load().gdn_gated_scan_fwd_sm100, "gdn_gated_scan_fwd_sm100", args, x.device)
     return o

@@ -15,7 +15,7 @@ import operator
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _check_device, _launch, _status_ptr
+from .ops import _DTYPES, _check_device, _empty, _launch, _status_ptr
 
 __all__ = ["window_attention", "window_attention_step"]
 
@@ -100,7 +100,7 @@ def window_attention(q, k, v, window, sinks=0, *, scale=None, lengths=None):
         _check_device("lengths", lengths, dev, "q")
     for name, t in tensors:
         _check_device(name, t, dev, "q")
-    o = torch.empty((B, T, H, D), dtype=q.dtype, device=dev)
+    o = _empty(q, q.dtype)
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), o.stride()
     args = _lib.WINDOW_ATTN_ARGS.pack(
         # beyond the keys neither window nor sinks change anything
@@ -159,7 +159,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, window, sinks=0,
     for name, t in tensors:
         _check_device(name, t, dev, "q")
     _check_device("positions", positions, dev, "q")
-    o = torch.empty((B, H, D), dtype=q.dtype, device=dev)
+    o = _empty(q, q.dtype)
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), o.stride()
     args = _lib.WINDOW_STEP_ARGS.pack(
         _lib.ABI_VERSION, B, H, HK, D, cap, window, sinks, _DTYPES[q.dtype], scale,
