@@ -16,12 +16,19 @@
 // neighbouring tiles of one head.  So every K/V tile fetched feeds two
 // products, and while one tile's softmax runs the tensor core works on the
 // other's.  One CTA per SM takes item after item; its loads and first scores
-// of the next item run under the last one's epilogue.  Warps: 2 x 8 softmax
-// (two threads per query row, 32 of a tile's 64 keys each), one that fetches
-// tiles by TMA, two that issue the MMAs (one for each query tile: issuing, at 35 cycles
-// an instruction, takes longer than the products).  TMEM holds two score buffers and the
-// output of both query tiles; the probabilities overwrite their scores' columns
-// and are the second product's TMEM operand, so they never touch shared memory.
+// of the next item run under the last one's epilogue.  Warps: 2 x 4 softmax
+// (a thread per query row), one that fetches tiles by TMA, two that issue the
+// MMAs (one for each query tile).  TMEM holds two score buffers of 64 keys and
+// the output of both query tiles; the probabilities overwrite their scores'
+// columns and are the second product's TMEM operand, so they never touch shared
+// memory.
+//
+// What was tried: 128-key tiles with one score buffer leave the softmax waiting
+// for both products (1119 us at 16384 tokens, 32 query and 8 key heads of 128,
+// window 4096, against 851); two threads per row, to have more warps to switch
+// between, cost more instructions than they hide (922); a quarter of the
+// exponentials as polynomials on the FMA pipe gain nothing (868).  A spilled
+// register costs dearly: with this much shared memory taken, local memory is L2.
 //
 // Masks.  Only tiles that some mask cuts are masked element by element.  In
 // those a key hidden from a row has probability 0, and 0 times a value that is
@@ -46,14 +53,10 @@ namespace {
 
 constexpr int kTile = 128;          // query rows per tile
 constexpr int kKeys = 64;           // keys per tile
-constexpr int kSoftmaxWarps = 16;   // 8 per query tile: 4 lane quarters x 2 halves of the keys
-constexpr int kTmaWarp = 16, kMmaWarp = 17;  // and kMmaWarp + 1: a query tile's products each
-// Five warpgroups, so that registers can be moved between them: 96 each at
-// launch, then 4 x 104 for the softmax warps and 64 for the others (480 in all).
-constexpr int kThreads = 20 * 32;
-// Named barriers: 1, 2 a query tile's group; 3 all warps; 4 .. 11 the two warps that share rows.
-constexpr int kBarGroup = 1, kBarAll = 3, kBarPair = 4;
-constexpr int kPolyPairs = 4;       // of a thread's 16 pairs of exponentials: on the FMA pipe (none: 953 us, 4: 887, 8: 966)
+constexpr int kSoftmaxWarps = 8;    // 4 per query tile
+constexpr int kTmaWarp = 8, kMmaWarp = 9;  // and kMmaWarp + 1: a query tile's products each
+constexpr int kThreads = 11 * 32;
+constexpr int kBarGroup = 1, kBarAll = 3;  // named barriers: 1 and 2 a query tile's group, 3 all warps
 constexpr int kMaxItems = 8192;     // of one CTA
 constexpr uint32_t kTmCols = 512;
 constexpr uint32_t kTmS = 0, kTmO = 256;  // + 128 x tile (+ 64 x buffer of the scores)
@@ -79,9 +82,8 @@ struct Lay {
   static constexpr uint32_t stage = 2 * kvtile;           // one two on: what the MMA warp takes in one step
   static constexpr uint32_t q = 0;                        // two query tiles
   static constexpr uint32_t kv = 2 * qtile;
-  static constexpr uint32_t out = kv + stages * stage;    // [16 warps][32 rows][16 columns] of outputs
-  static constexpr uint32_t red = out + 16384;            // [2][2][2][128] row maxima (two in turn), sums
-  static constexpr uint32_t bars = red + 4096;
+  static constexpr uint32_t out = kv + stages * stage;    // [8 warps][32 rows][16 columns] of outputs
+  static constexpr uint32_t bars = out + 8192;
   static constexpr uint32_t misc = bars + 8 * (2 * stages + 20);
   static constexpr uint32_t redo = misc + 64;             // one bit per item of this CTA
   static constexpr uint32_t bytes = redo + kMaxItems / 8;
@@ -178,38 +180,12 @@ __device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
   return r;
 }
 
-// 2^x on the FMA pipe, for the share of the exponentials that the special-function
-// pipe (16 per clock and SM) has no time for.  Cody-Waite: x = n + r with
-// |r| <= 1/2 by adding and subtracting 1.5 2^23, a polynomial of degree 4 for 2^r
-// (fitted for the least relative error, 2.6e-6, far below the 16-bit rounding
-// that follows), and n added to the exponent.  x <= 127; below -126, and for a
-// hidden key's -infinity, exactly 0: its value may be anything.
-__device__ __forceinline__ float2 exp2_poly(F2 x) {
-  float2 c = f2_get(x);
-  c.x = fmaxf(c.x, -126.f);
-  c.y = fmaxf(c.y, -126.f);
-  const F2 m = f2(c.x, c.y);
-  const F2 z = f2_add(m, f2(12582912.f, 12582912.f));
-  const F2 n = f2_add(z, f2(-12582912.f, -12582912.f));
-  const F2 r = f2_fma(n, f2(-1.f, -1.f), m);
-  F2 y = f2_fma(f2(0.00957016088f, 0.00957016088f), r, f2(0.0559178293f, 0.0559178293f));
-  y = f2_fma(y, r, f2(0.240247428f, 0.240247428f));
-  y = f2_fma(y, r, f2(0.693121791f, 0.693121791f));
-  y = f2_fma(y, r, f2(0.999999285f, 0.999999285f));
-  const float2 yy = f2_get(y), zz = f2_get(z);
-  return make_float2(c.x > -126.f ? __uint_as_float(__float_as_uint(yy.x) + (__float_as_uint(zz.x) << 23)) : 0.f,
-                     c.y > -126.f ? __uint_as_float(__float_as_uint(yy.y) + (__float_as_uint(zz.y) << 23)) : 0.f);
-}
-
 // The larger of three; NaN if one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-
-template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename T> struct Pair;
 template <> struct Pair<__half> {
@@ -266,8 +242,10 @@ struct Item {
 
 __device__ __forceinline__ Item make_item(const Params& P, int i) {
   Item it;
-  const int y = i / P.nx;
-  it.row0 = (i - y * P.nx) * (P.pair_heads ? kTile : 2 * kTile);
+  // Row tiles from the last to the first: early rows see fewer keys, and short
+  // items at the end fill the last round.
+  const int nb = P.items / P.nx, x = i / nb, y = i - x * nb;
+  it.row0 = (P.nx - 1 - x) * (P.pair_heads ? kTile : 2 * kTile);
   it.b = y / P.ny;
   it.hy = (y - it.b * P.ny) * (P.pair_heads ? 2 : 1);
   it.hk = it.hy / P.G;
@@ -301,19 +279,17 @@ __device__ __forceinline__ uint32_t tmem_ld1w(uint32_t taddr) {
 
 // O (+)= P V of one key tile over this row's visible keys alone, on the CUDA
 // cores: for tiles whose values are not all finite.  P is read back from TMEM.
-// Each of a row's two threads takes half the columns (tm_o: its first).
 template <typename T, int D>
-__device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uint8_t* vt, int half, bool first, int k0,
+__device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uint8_t* vt, bool first, int k0,
                                          int last, int behind, int sinks) {
-  for (int c1 = 0; c1 < D / 2; c1 += 32) {
-    const int c0 = half * (D / 2) + c1;
+  for (int c0 = 0; c0 < D; c0 += 32) {
     float o[32];
     uint32_t ou[32];
     if (first) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) o[i] = 0.f;
     } else {
-      tmem_ld32w(tm_o + c1, o);
+      tmem_ld32w(tm_o + c0, o);
     }
     for (int j = 0; j < kKeys; ++j) {
       const float2 pp = Cvt<T>::unpack(tmem_ld1w(tm_p + (j >> 1)));
@@ -340,12 +316,12 @@ __device__ __noinline__ void sum_visible(uint32_t tm_p, uint32_t tm_o, const uin
     }
 #pragma unroll
     for (int i = 0; i < 32; ++i) ou[i] = __float_as_uint(o[i]);
-    tmem_st32(tm_o + c1, ou);
+    tmem_st32(tm_o + c0, ou);
     tmem_wait_st();
   }
 }
 
-// Masked scores of half a tile: this row's visible keys are those up to hi, from lo on or below sk.
+// Masked scores of 32 keys: this row's visible keys are those up to hi, from lo on or below sk.
 __device__ __forceinline__ void mask_row(float* s, int hi, int lo, int sk) {
   // bits of the columns < n
   auto below = [](int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); };
@@ -424,7 +400,6 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   bool ok = true;
 
   if (warp >= kSoftmaxWarps) {
-    regs_less<64>();
     bool careful = false;
     do {
       if (warp == kTmaWarp) {
@@ -519,16 +494,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       }
     } while (careful = again(careful), careful);
   } else {
-    regs_more<104>();
-    // ------------------------------------------------ softmax: two threads per query row of tile x
+    // ------------------------------------------------ softmax: thread = one query row of tile x
     // After an abort a warp runs on without waiting or computing, so that the
     // group's barriers still meet.
-    const int x = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
+    const int x = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = uint32_t(quarter * 32) << 16;
-    const uint32_t tm_s0 = tmem + lane_base + kTmS + x * 128, tm_o = tmem + lane_base + kTmO + x * 128 + half * (D / 2);
-    const int pair = kBarPair + x * 4 + quarter;
-    float* red = reinterpret_cast<float*>(sm + L::red) + x * 256 + r;  // [turn][x][half][row]
+    const uint32_t tm_s0 = tmem + lane_base + kTmS + x * 128, tm_o = tmem + lane_base + kTmO + x * 128;
     const float sl2 = P.scale_log2;
     // Two copies of the loop: the careful one's calls would cost the other its registers.
     auto softmax_pass = [&](auto kind) {
@@ -550,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           if (!rows.used()) {
             if (it.row(P, x) + r < P.T) {
               T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_t * (long long)(it.row(P, x) + r) + P.so_h * it.head(P, x);
-              for (int c = half; c < D / 8; c += 2) reinterpret_cast<uint4*>(op)[c] = make_uint4(0, 0, 0, 0);
+              for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(op)[c] = make_uint4(0, 0, 0, 0);
             }
             continue;
           }
@@ -563,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           all_to = (rows.p0 < len - 1 ? rows.p0 : len - 1) - (kKeys - 1);
           all_from = rows.p1 - P.window;
         }
-        float m = -INFINITY, l = 0.f;  // running reference maximum (raw scores); sum over this half
+        float m = -INFINITY, l = 0.f;  // running reference maximum (raw scores); sum
 #pragma unroll 1
         for (int t = 0; t < tiles; ++t) {
           const int k0 = t < n_sink ? t * kKeys : from + (t - n_sink) * kKeys;
@@ -571,34 +543,30 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           const uint32_t buf = ns0 & 1, before = (ns0 - 1) & 1;
           const uint32_t tm_s = tm_s0 + buf * 64;
           if (ok) ok = mbar_wait_warp(&bars[B_S + 2 * x + buf], (ns0 >> 1) & 1, abort_flag);
-          float s[32];
+          float s[64];
           float mt = 0.f;
           if (ok) {
             tc_fence_after();
-            tmem_ld32w(tm_s + 32 * half, s);
+            tmem_ld32x2w(tm_s, s, tm_s + 32, s + 32);
             if (cut) {
-              const int c0 = k0 + 32 * half;
-              mask_row(s, (p < len ? p : -1) - c0, p - P.window + 1 - c0, P.sinks - c0);  // rows behind the sequence see none
+              const int hi = p < len ? p : -1;
+              mask_row(s, hi - k0, p - P.window + 1 - k0, P.sinks - k0);
+              mask_row(s + 32, hi - k0 - 32, p - P.window + 1 - k0 - 32, P.sinks - k0 - 32);  // rows behind the sequence see none
             }
             // a NaN among the scores becomes the maximum, and so the row's output
             float mx[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[4 + e], s[8 + e]);
 #pragma unroll
-            for (int c = 12; c < 28; c += 8)
+            for (int c = 12; c < 60; c += 8)
 #pragma unroll
               for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[28 + e], s[28 + e]);
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[60 + e], s[60 + e]);
             mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-            red[buf * 512 + half * 128] = mt;
           }
-          // Both halves have their scores and know each other's maximum from here on.
-          named_bar(pair, 64);
           ++ns0;
           if (ok) {
-            const float mo = red[buf * 512 + (half ^ 1) * 128];
-            mt = max3(mt, mo, mo);
             // The reference follows the maximum only when a probability would
             // pass 2^8: most tiles then leave O as it is.
             const bool up = !((mt - m) * sl2 <= 8.f) && mt != -INFINITY;
@@ -612,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
                 if (ok) {
                   tc_fence_after();
 #pragma unroll 1
-                  for (int c = 0; c < D / 2; c += 16) {
+                  for (int c = 0; c < D; c += 16) {
                     float o[16];
                     tmem_ld16w(tm_o + c, o);
                     uint32_t ou[16];
@@ -626,18 +594,21 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
             const float ms = m == -INFINITY ? 0.f : m * sl2;
             const F2 sl = f2(sl2, sl2), nm = f2(-ms, -ms);
             F2 sum0 = f2(0.f, 0.f), sum1 = sum0;
-            uint32_t pk[16];
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              float2 e = f2_get(f2_fma(f2(s[2 * c], s[2 * c + 1]), sl, nm));
-              e = c < kPolyPairs ? exp2_poly(f2(e.x, e.y)) : make_float2(fast_exp2(e.x), fast_exp2(e.y));
-              if (c & 1)
-                sum1 = f2_add(sum1, f2(e.x, e.y));
-              else
-                sum0 = f2_add(sum0, f2(e.x, e.y));
-              pk[c] = Cvt<T>::pack(e.x, e.y);
+            for (int h = 0; h < 2; ++h) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                float2 e = f2_get(f2_fma(f2(s[32 * h + 2 * c], s[32 * h + 2 * c + 1]), sl, nm));
+                e = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                if (c & 1)
+                  sum1 = f2_add(sum1, f2(e.x, e.y));
+                else
+                  sum0 = f2_add(sum0, f2(e.x, e.y));
+                pk[c] = Cvt<T>::pack(e.x, e.y);
+              }
+              tmem_st16(tm_s + 16 * h, pk);
             }
-            tmem_st16(tm_s + 16 * half, pk);
             const float2 sum = f2_get(f2_add(sum0, sum1));
             l += sum.x + sum.y;
             tmem_wait_st();
@@ -652,13 +623,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
               if (ok && t > 0) ok = mbar_wait_warp(&bars[B_V + x], before, abort_flag);
               tc_fence_before();
               // (the barrier is also where both halves' probabilities meet)
-              slow = bar_any(kBarGroup + x, 256, ok && half == 0 && r < kKeys && row_not_finite<T, D>(vt, r));
+              slow = bar_any(kBarGroup + x, 128, ok && r < kKeys && row_not_finite<T, D>(vt, r));
               if (slow && ok) {
                 tc_fence_after();
-                sum_visible<T, D>(tm_s, tm_o, vt, half, t == 0, k0, p < len ? p : -1, p - P.window, P.sinks);
+                sum_visible<T, D>(tm_s, tm_o, vt, t == 0, k0, p < len ? p : -1, p - P.window, P.sinks);
               }
             }
-            if (ok && half == 0 && r == 0) skip_pv[2 * x + buf] = slow;
+            if (ok && r == 0) skip_pv[2 * x + buf] = slow;
             __threadfence_block();
           }
           if (ok) {
@@ -669,10 +640,6 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
         }
         // -------------------------------------------- o = O / l
         if (ok) ok = mbar_wait_warp(&bars[B_O + x], nq0 & 1, abort_flag);
-        red[(ns0 & 1) * 512 + half * 128] = l;
-        named_bar(pair, 64);
-        l += red[(ns0 & 1) * 512 + (half ^ 1) * 128];
-        named_bar(pair, 64);  // read before the next item's maxima
         if (ok) {
           tc_fence_after();
           const Item it = make_item(P, i);
@@ -682,12 +649,12 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           // Rows leave through shared memory, so that a store covers whole sectors.
           uint8_t* stage = sm + L::out + warp * 1024;
           const int row = it.row(P, x) + quarter * 32;  // this warp's first
-          T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_h * it.head(P, x) + P.so_t * (long long)row + half * (D / 2);
+          T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_h * it.head(P, x) + P.so_t * (long long)row;
 #pragma unroll 1
-          for (int part = 0; part < D / 32; ++part) {
+          for (int part = 0; part < D / 16; ++part) {
             float o[16];
             tmem_ld16w(tm_o + 16 * part, o);
-            if (part == D / 32 - 1) {
+            if (part == D / 16 - 1) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&bars[B_OE + x]);
