@@ -82,8 +82,8 @@ struct Lay {
   static constexpr uint32_t stage = 2 * kvtile;           // one two on: what the MMA warp takes in one step
   static constexpr uint32_t q = 0;                        // two query tiles
   static constexpr uint32_t kv = 2 * qtile;
-  static constexpr uint32_t out = kv + stages * stage;    // [8 warps][32 rows][16 columns] of outputs
-  static constexpr uint32_t bars = out + 8192;
+  static constexpr uint32_t out = kv + stages * stage;    // [8 warps][32 rows][32 columns] of outputs
+  static constexpr uint32_t bars = out + 16384;
   static constexpr uint32_t misc = bars + 8 * (2 * stages + 20);
   static constexpr uint32_t redo = misc + 64;             // one bit per item of this CTA
   static constexpr uint32_t bytes = redo + kMaxItems / 8;
@@ -622,7 +622,6 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
               if (ok) ok = mbar_wait_warp(&full[n % L::stages], (n / L::stages) & 1, abort_flag);
               if (ok && t > 0) ok = mbar_wait_warp(&bars[B_V + x], before, abort_flag);
               tc_fence_before();
-              // (the barrier is also where both halves' probabilities meet)
               slow = bar_any(kBarGroup + x, 128, ok && r < kKeys && row_not_finite<T, D>(vt, r));
               if (slow && ok) {
                 tc_fence_after();
@@ -647,20 +646,20 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           const float inv = 1.f / l;
           float odd = 0.f;  // NaN if some output is not finite
           // Rows leave through shared memory, so that a store covers whole sectors.
-          uint8_t* stage = sm + L::out + warp * 1024;
+          uint8_t* stage = sm + L::out + warp * 2048;
           const int row = it.row(P, x) + quarter * 32;  // this warp's first
           T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_h * it.head(P, x) + P.so_t * (long long)row;
 #pragma unroll 1
-          for (int part = 0; part < D / 16; ++part) {
-            float o[16];
-            tmem_ld16w(tm_o + 16 * part, o);
-            if (part == D / 16 - 1) {
+          for (int part = 0; part < D / 32; ++part) {
+            float o[32];
+            tmem_ld32w(tm_o + 32 * part, o);
+            if (part == D / 32 - 1) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&bars[B_OE + x]);
             }
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < 4; ++c) {
               uint4 w;
               uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
@@ -670,15 +669,14 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
                 odd = fmaf(b2, 0.f, odd);
                 wp[e] = live ? Cvt<T>::pack(a, b2) : 0u;
               }
-              // rows of 32 bytes, their two pieces swapped every fourth row
-              *reinterpret_cast<uint4*>(stage + lane * 32 + ((c ^ ((lane >> 2) & 1)) << 4)) = w;
+              *reinterpret_cast<uint4*>(stage + sw64_off(lane, c)) = w;
             }
             __syncwarp();
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int rr = 16 * c + (lane >> 1);
-              const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 32 + (((lane & 1) ^ ((rr >> 2) & 1)) << 4));
-              if (row + rr < P.T) reinterpret_cast<uint4*>(op + P.so_t * (long long)rr + 16 * part)[lane & 1] = w;
+            for (int c = 0; c < 4; ++c) {
+              const int rr = 8 * c + (lane >> 2);
+              const uint4 w = *reinterpret_cast<const uint4*>(stage + sw64_off(rr, lane & 3));
+              if (row + rr < P.T) reinterpret_cast<uint4*>(op + P.so_t * (long long)rr + 32 * part)[lane & 3] = w;
             }
             __syncwarp();
           }
@@ -798,7 +796,7 @@ int run(const gdn_window_attn_args* a, void* stream) {
   p.nx = (a->T + rows - 1) / rows;
   p.ny = p.pair_heads ? a->H / 2 : a->H;
   const long long items = (long long)p.nx * p.ny * a->B;
-  if (items > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED;
+  if (items > 0x7fff0000LL) return GDN_ERR_UNSUPPORTED;
   p.items = int(items);
   int sms = 0;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return cuda_failed();
