@@ -216,6 +216,33 @@ def test_strides_and_views():
             assert torch.equal(u, v)
 
 
+@pytest.mark.parametrize("size", [(40, 300, 4, 128), (3, 1400, 2, 512), (2, 300, 3, 200)], ids=str)
+def test_wide_and_head_first_layouts(size):
+    """Many chains, heads wider than a CTA's columns, and storage with the heads before the time."""
+    import gdn_b200
+    x, g, h0, do, dh = make(*size, seed=9)
+    a, h0r, h, s, e = reference(x, g, h0, False)
+    want = None
+    for first in (lambda t: t, lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)):
+        xl, gl = first(x).requires_grad_(), first(g).requires_grad_()
+        o, hT = gdn_b200.gated_scan(xl, gl, h0)
+        check("o", o, h, e)
+        check("hT", hT, h[:, -1], e[:, -1])
+        got = (o.detach(), hT.detach()) + torch.autograd.grad((o, hT), (xl, gl), (do.to(o.dtype), dh))
+        want = want or got
+        assert all(torch.equal(u, w) for u, w in zip(got, want))
+
+
+def test_one_tensor_as_both_inputs():
+    import gdn_b200
+    z = -torch.rand(1, 80, 1, 64, device="cuda")
+    zl = z.clone().requires_grad_()
+    (both,) = torch.autograd.grad(gdn_b200.gated_scan(zl, zl)[0].sum(), zl)
+    x, g = z.clone().requires_grad_(), z.clone().requires_grad_()
+    dx, dg = torch.autograd.grad(gdn_b200.gated_scan(x, g)[0].sum(), (x, g))
+    assert torch.equal(both, dx + dg)
+
+
 def test_resets_and_extreme_gates():
     """-inf resets the chain, 0 keeps it, saturated logits do either; gradients stay finite."""
     import gdn_b200

@@ -86,6 +86,8 @@ SIZES = [
     (1, 777, 777, 5, 1, 128, 4096, 0),
     (1, 1030, 1030, 2, 1, 64, 127, 300),
     (1, 640, 3000, 2, 1, 128, 1500, 64),
+    (1, 300, 333, 2, 1, 64, 1, 10000),
+    (2, 70, 4000, 1, 1, 128, 3, 65),
 ]
 
 
@@ -167,6 +169,21 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(dt, what):
         col = got[:, 5]
         assert torch.equal(col.isnan(), nan)
         assert torch.equal(col == math.inf, pos & ~nan) and torch.equal(col == -math.inf, neg & ~nan)
+
+
+def test_many_items_per_cta_with_poisoned_ones():
+    """More work items than SMs, some of them done twice: each as if it were alone, bit for bit."""
+    import gdn_b200
+    B, T, H, HK, D = 10, 900, 8, 8, 64
+    q, k, v = make(B, T, T, H, HK, D, torch.bfloat16, 12)
+    for b, j, h in ((0, 899, 0), (3, 450, 2), (3, 451, 2), (7, 0, 5), (9, 130, 7)):
+        v[b, j, h, j % D] = float("nan") if j % 2 else float("inf")
+    k[5, 600, 1] = float("nan")
+    o = gdn_b200.window_attention(q, k, v, 170, 3)
+    gdn_b200.check_status()
+    for b in range(B):
+        one = gdn_b200.window_attention(q[b:b + 1], k[b:b + 1], v[b:b + 1], 170, 3)
+        assert torch.equal(one[0].view(torch.int16), o[b].view(torch.int16)), b
 
 
 def test_large_scores_and_growing_maxima():
