@@ -30,6 +30,11 @@
 // exponentials as polynomials on the FMA pipe gain nothing (868).  A spilled
 // register costs dearly: with this much shared memory taken, local memory is L2.
 //
+// The probabilities are rounded once to the operands' type, as the 16-bit product
+// has to have them: that adds as much as the output's own rounding (the sum of
+// the two against 64 bits: 1.3 to 1.4 times the latter).  Scores, maxima, sums and
+// outputs are fp32.
+//
 // Masks.  Only tiles that some mask cuts are masked element by element.  In
 // those a key hidden from a row has probability 0, and 0 times a value that is
 // not finite would still poison the row.  Such an output cannot be missed: it is

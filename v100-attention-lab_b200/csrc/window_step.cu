@@ -15,13 +15,18 @@
 // straight into MMA fragments in 16-byte pieces: the products' inner index may
 // run in any order, so a lane's 16 contiguous bytes of a key are the fragments
 // of two steps, and for V the columns are dealt out so that a lane's 16 bytes
-// are its share of eight column tiles.  No staging in shared memory, and with
-// 16 warps of 8 KB loads in flight on an SM the loads cover their latency.
+// are its share of eight column tiles.  No staging in shared memory: the next
+// tile's keys are fetched into the registers of the current one's while its
+// softmax runs, its values under the next scores.
 // Running maxima, sums and outputs are joined warp by warp in shared memory and
 // CTA by CTA through distributed shared memory, in a fixed order.
 //
 // Probabilities enter the second product as the sum of two 16-bit terms: a
 // single rounding would cost as much as the output's own.
+//
+// Measured: 64 sequences, 32 query and 8 key heads of 128, 4100 keys (1.08 GB):
+// 206 us, 5.2 TB/s; without the overlapped fetch 290; with spilled registers
+// (16 warps on an SM instead of 8) 350.
 #include "../../include/gdn_b200.h"
 #include "host_util.h"
 #include "tc.cuh"

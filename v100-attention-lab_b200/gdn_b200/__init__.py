@@ -1,7 +1,9 @@
 """gdn_b200 -- B200-native chunked Gated DeltaNet forward (sm_100a).
 
 Drop-in for the forward entry point of 123123213weqw/v100-attention-lab
-(``gdn_triton.gdn_chunk_fwd``); see ``ops.gdn_chunk_fwd``.
+(``gdn_triton.gdn_chunk_fwd``); see ``ops.gdn_chunk_fwd``.  Beside it: the
+elementwise gated recurrence (``recurrence``), windowed attention (``windowed``)
+and the single-token forms of all three.
 """
 
 from .fla_compat import chunk_delta_rule, chunk_gated_delta_rule
