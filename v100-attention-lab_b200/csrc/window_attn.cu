@@ -76,6 +76,7 @@ struct Params {
   int window, sinks;
   int nx, ny, items;  // row tiles (or pairs) and heads (or pairs) of an item grid, items in all
   int pair_heads;    // an item's two tiles are two heads (else two row tiles of one head)
+  int single;        // an item is one tile, its second one empty
   float scale_log2;  // scale * log2(e)
 };
 
@@ -241,7 +242,8 @@ struct Item {
   __device__ __forceinline__ int head(const Params& P, int x) const { return hy + (P.pair_heads ? x : 0); }
   __device__ __forceinline__ Rows rows(const Params& P, int x) const {
     const int r = row(P, x);
-    return Rows{P.S - P.T + r, P.S - P.T + (r + kTile < P.T ? r + kTile : P.T) - 1, len, P.window, P.sinks};
+    const int p0 = P.S - P.T + r;
+    return Rows{p0, x && P.single ? p0 - 1 : P.S - P.T + (r + kTile < P.T ? r + kTile : P.T) - 1, len, P.window, P.sinks};
   }
 };
 
@@ -250,7 +252,7 @@ __device__ __forceinline__ Item make_item(const Params& P, int i) {
   // Row tiles from the last to the first: early rows see fewer keys, and short
   // items at the end fill the last round.
   const int nb = P.items / P.nx, x = i / nb, y = i - x * nb;
-  it.row0 = (P.nx - 1 - x) * (P.pair_heads ? kTile : 2 * kTile);
+  it.row0 = (P.nx - 1 - x) * (P.pair_heads || P.single ? kTile : 2 * kTile);
   it.b = y / P.ny;
   it.hy = (y - it.b * P.ny) * (P.pair_heads ? 2 : 1);
   it.hk = it.hy / P.G;
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           const Rows rows = it.rows(P, x);
           if (it.count > 0) nkv += it.count + 2;
           if (!rows.used()) {
-            if (it.row(P, x) + r < P.T) {
+            if (rows.p1 >= rows.p0 && it.row(P, x) + r < P.T) {
               T* op = static_cast<T*>(P.o) + P.so_b * it.b + P.so_t * (long long)(it.row(P, x) + r) + P.so_h * it.head(P, x);
               for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(op)[c] = make_uint4(0, 0, 0, 0);
             }
@@ -796,15 +798,19 @@ int run(const gdn_window_attn_args* a, void* stream) {
   p.window = a->window < a->S ? a->window : a->S;
   p.sinks = a->sinks < a->S ? a->sinks : a->S;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  p.pair_heads = p.G % 2 == 0;
-  const int rows = p.pair_heads ? kTile : 2 * kTile;
-  p.nx = (a->T + rows - 1) / rows;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return cuda_failed();
+  // Items of one tile where all of them run at once: a chunk of 3 x 501 rows, 12
+  // heads of 64, takes 15.8 us (18.2 in items of two).  With more items than SMs
+  // two tiles share the keys fetched, and one's softmax runs under the other's products.
+  const int tiles = (a->T + kTile - 1) / kTile;
+  p.single = (long long)tiles * a->H * a->B <= sms;
+  p.pair_heads = !p.single && p.G % 2 == 0;
+  p.nx = p.single || p.pair_heads ? tiles : (tiles + 1) / 2;
   p.ny = p.pair_heads ? a->H / 2 : a->H;
   const long long items = (long long)p.nx * p.ny * a->B;
   if (items > 0x7fff0000LL) return GDN_ERR_UNSUPPORTED;
   p.items = int(items);
-  int sms = 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return cuda_failed();
   // one CTA per SM, more only where one could not note all its items
   long long ctas = (items + kMaxItems - 1) / kMaxItems;
   if (ctas < sms) ctas = items < sms ? items : sms;

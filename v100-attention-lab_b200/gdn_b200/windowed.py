@@ -9,7 +9,6 @@ sm_100a library through its C ABI.
 
 from __future__ import annotations
 
-import math
 import operator
 
 import torch
@@ -20,34 +19,42 @@ from .ops import _DTYPES, _check_device, _empty, _launch, _status_ptr
 __all__ = ["window_attention", "window_attention_step"]
 
 
-def _check(tensors, D, window, sinks, scale):
-    """Checks that both entry points share; returns the scale."""
-    q = tensors[0][1]
-    dtype = q.dtype
+def _check_tensors(tensors):
+    """Types, layouts and gradients of the tensors; their common type is the first's."""
     grad = torch.is_grad_enabled()
+    dtype = None
     for name, t in tensors:
-        if t.dtype != dtype:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if dtype is None:
+            dtype = t.dtype
+        elif t.dtype != dtype:
             raise ValueError(f"{name} must have q's dtype (got {t.dtype}, q has {dtype})")
         if t.stride(-1) != 1:
             raise ValueError(f"{name} must have a contiguous last dimension")
         if grad and t.requires_grad:
             raise NotImplementedError("windowed attention has no backward: call it under torch.no_grad()")
-    if dtype not in (torch.float16, torch.bfloat16):
+    if dtype != torch.bfloat16 and dtype != torch.float16:
         raise NotImplementedError(f"gdn_b200 takes fp16 or bf16 q/k/v (got {dtype})")
+
+
+def _check_sizes(D, window, sinks, scale):
+    """Head size, window and sinks; returns the scale."""
     if D != 64 and D != 128:
         raise NotImplementedError(f"the head size must be 64 or 128 (got {D})")
     if window < 1 or sinks < 0:
         raise ValueError(f"window must be at least 1 and sinks at least 0 (got {window}, {sinks})")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 1e30:
         raise ValueError(f"scale must be positive (got {scale})")
     return scale
 
 
-def _check_tensors(tensors):
+def _check_devices(tensors, dev):
+    """All CUDA tensors on ``dev``, the device of the first."""
     for name, t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.device != dev or not t.is_cuda:
+            _check_device(name, t, dev, "q")
 
 
 def _check_ints(name, t, B):
@@ -93,13 +100,12 @@ def window_attention(q, k, v, window, sinks=0, *, scale=None, lengths=None):
     if S < T:
         raise ValueError(f"fewer keys ({S}) than query rows ({T})")
     window, sinks = operator.index(window), operator.index(sinks)
-    scale = _check(tensors, D, window, sinks, scale)
+    scale = _check_sizes(D, window, sinks, scale)
     dev = q.device
     if lengths is not None:
         _check_ints("lengths", lengths, B)
         _check_device("lengths", lengths, dev, "q")
-    for name, t in tensors:
-        _check_device(name, t, dev, "q")
+    _check_devices(tensors, dev)
     o = _empty(q, q.dtype)
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), o.stride()
     args = _lib.WINDOW_ATTN_ARGS.pack(
@@ -147,7 +153,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, window, sinks=0,
     if H % HK != 0:
         raise ValueError(f"the number of query heads ({H}) must be a multiple of the key heads ({HK})")
     window, sinks = operator.index(window), operator.index(sinks)
-    scale = _check(tensors, D, window, sinks, scale)
+    scale = _check_sizes(D, window, sinks, scale)
     if window + sinks > cap:
         raise ValueError(f"the cache's capacity ({cap}) must hold window + sinks ({window + sinks}) tokens")
     skc, svc = k_cache.stride(), v_cache.stride()
@@ -156,8 +162,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, window, sinks=0,
             raise ValueError(f"{name} is written to and must not be an expanded tensor")
     _check_ints("positions", positions, B)
     dev = q.device
-    for name, t in tensors:
-        _check_device(name, t, dev, "q")
+    _check_devices(tensors, dev)
     _check_device("positions", positions, dev, "q")
     o = _empty(q, q.dtype)
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), o.stride()
