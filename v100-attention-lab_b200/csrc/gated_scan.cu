@@ -796,7 +796,7 @@ bool elem_aligned(const void* ptr, int es) { return reinterpret_cast<uintptr_t>(
 int validate(const gdn_gated_scan_args* a, Pass pass) {
   if (a == nullptr || a->abi_version != GDN_B200_ABI_VERSION) return GDN_ERR_INVALID_ARGUMENT;
   if (a->B < 1 || a->T < 1 || a->H < 1 || a->D < 1) return GDN_ERR_INVALID_ARGUMENT;
-  if ((long long)a->H * a->D > 0x3fffffffLL || (long long)a->T > 0x7fffff00LL) return GDN_ERR_UNSUPPORTED;
+  if ((long long)a->H * a->D > 0x3fffffffLL || a->T > 0x7fff0000) return GDN_ERR_UNSUPPORTED;
   if ((long long)a->B * a->H * a->D > 0x1fffffffffLL) return GDN_ERR_UNSUPPORTED;
   if (a->flags & ~GDN_FLAG_G_LOGSIGMOID) return GDN_ERR_INVALID_ARGUMENT;
   for (int dt : {a->x_dtype, a->g_dtype, a->o_dtype})
