@@ -31,9 +31,10 @@
 // register costs dearly: with this much shared memory taken, local memory is L2.
 //
 // The probabilities are rounded once to the operands' type, as the 16-bit product
-// has to have them: that adds as much as the output's own rounding (the sum of
-// the two against 64 bits: 1.3 to 1.4 times the latter).  Scores, maxima, sums and
-// outputs are fp32.
+// has to have them.  Where keys of like weight make up the output that adds as
+// much as the output's own rounding (the sum of the two against 64 bits, for
+// normally distributed scores: 1.3 to 1.4 times the latter); fp16 adds its grid
+// (see kSlack) for keys far below the largest.  Scores, maxima, sums and outputs are fp32.
 //
 // Masks.  Only tiles that some mask cuts are masked element by element.  In
 // those a key hidden from a row has probability 0, and 0 times a value that is
@@ -48,6 +49,7 @@
 
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <type_traits>
@@ -78,6 +80,7 @@ struct Params {
   int pair_heads;    // an item's two tiles are two heads (else two row tiles of one head)
   int single;        // an item is one tile, its second one empty
   float scale_log2;  // scale * log2(e)
+  float shift;       // log2 of the scale of a probability at the reference
 };
 
 template <int D>
@@ -160,6 +163,22 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// How far (log2) a row's probabilities may pass 1 before its reference follows
+// the maximum, and the scale that they get before they are rounded, which the sum
+// shares, so that it cancels.  fp16 has a grid of 2^-24 and ends at 2^16: with the
+// reference at 2^11 a probability is exact to 2^-36, or to its own half step (at
+// 1, with a slack of 8, keys 15 nats below a dominant sink were 8 half steps off
+// and those 18 below it lost); a factor of 2 is left for the exponent's rounding at
+// scores of millions.  A smaller slack has O scaled more often: a call of 1x16384
+// tokens, 32/8 heads of 128, window 4096, takes 985 to 996 us at 8 and at 4 alike,
+// 1013 at 3, 1071 at 2.  bf16 keeps its accuracy at any scale: it takes the slack and the number of
+// keys back, so that sums of values near the end of fp32's range stay in it, as
+// their average does.
+template <typename T> constexpr float kSlack = Cvt<T>::kIsBf16 ? 8.f : 4.f;
+float shift_of(int dtype, long long keys) {
+  return dtype == GDN_DTYPE_F16 ? 11.f : -kSlack<__nv_bfloat16> - float(std::ceil(std::log2(double(keys))));
+}
 
 // Two fp32 operations in one instruction.
 struct F2 {
@@ -575,8 +594,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           ++ns0;
           if (ok) {
             // The reference follows the maximum only when a probability would
-            // pass 2^8: most tiles then leave O as it is.
-            const bool up = !((mt - m) * sl2 <= 8.f) && mt != -INFINITY;
+            // pass the slack: most tiles then leave O as it is.
+            const bool up = !((mt - m) * sl2 <= kSlack<T>) && mt != -INFINITY;
             if (__any_sync(0xffffffffu, up)) {
               const float corr = !up ? 1.f : (m == -INFINITY ? 0.f : fast_exp2((m - mt) * sl2));
               if (up) m = mt == INFINITY ? NAN : mt;  // infinity less infinity
@@ -599,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
               }
             }
             const float ms = m == -INFINITY ? 0.f : m * sl2;
-            const F2 sl = f2(sl2, sl2), nm = f2(-ms, -ms);
+            const F2 sl = f2(sl2, sl2), nm = f2(P.shift - ms, P.shift - ms);
             F2 sum0 = f2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -798,6 +817,8 @@ int run(const gdn_window_attn_args* a, void* stream) {
   p.window = a->window < a->S ? a->window : a->S;
   p.sinks = a->sinks < a->S ? a->sinks : a->S;
   p.scale_log2 = a->scale * 1.4426950408889634f;
+  const long long keys = (long long)p.window + p.sinks;  // that a row sees
+  p.shift = shift_of(a->dtype, keys < a->S ? keys : a->S);
   int sms = 0;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return cuda_failed();
   // Items of one tile where all of them run at once: a chunk of 3 x 501 rows, 12
