@@ -114,3 +114,37 @@ def test_bf16_values_near_the_end_of_the_range_one_token(size):
     o = gdn_b200.window_attention_step(q[:, p], k[:, p], v[:, p], kc, vc, pos, window, sinks)
     n = min(S, window + sinks)
     compare("o", o, ref[p:], tolerance(ref[p:], mag[p:], reach[p:], q.dtype, D, n, 1 / math.sqrt(D), 3e38, True))
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [(2, 4, 2, 64, 20, 2), (1, 20, 1, 128, 700, 4), (3, 6, 2, 128, 90, 0)], ids=str)
+def test_infinities_that_one_token_sees(dt, size):
+    """inf and -inf come out as such, both or a NaN as NaN, in their columns and heads alone."""
+    import gdn_b200
+    B, H, HK, D, window, sinks = size
+    cap = window + sinks + 3
+    q, k, v = make(B, 1, 1, H, HK, D, TYPES[dt], 6)
+    kc, vc = make(B, cap, cap, HK, HK, D, TYPES[dt], 7)[1:]
+    p = 3 * cap + 1
+    seen = list(range(sinks)) + list(range(p - window + 1, p + 1))
+    slots = [slot(j, cap, sinks) for j in seen]
+    hidden = sorted(set(range(cap)) - set(slots))
+    pos = torch.full((B,), p, dtype=torch.int32, device="cuda")
+    clean = gdn_b200.window_attention_step(q[:, 0], k[:, 0], v[:, 0], kc, vc, pos, window, sinks)
+    inf = float("inf")
+    vc[:, hidden] = float("nan")
+    v[:, 0, 0, 9], v[:, 0, 0, 21] = inf, inf          # the token's own value
+    vc[:, slots[0], 0, 5] = inf
+    vc[:, slots[3], 0, 6], vc[:, slots[-2], 0, 6] = -inf, -inf
+    vc[:, slots[4], 0, 7], vc[:, slots[-3], 0, 7] = inf, -inf
+    vc[:, slots[5], 0, 8] = float("nan")
+    vc[:, slots[1], 0, 21] = -inf
+    o = gdn_b200.window_attention_step(q[:, 0], k[:, 0], v[:, 0], kc, vc, pos, window, sinks)
+    G = H // HK
+    assert torch.equal(o[:, G:], clean[:, G:])
+    rest = [d for d in range(D) if d not in (5, 6, 7, 8, 9, 21)]
+    assert torch.equal(o[..., rest], clean[..., rest])
+    got = o[:, :G]
+    assert (got[..., 5] == inf).all() and (got[..., 9] == inf).all()
+    assert (got[..., 6] == -inf).all()
+    assert got[..., [7, 8, 21]].isnan().all()

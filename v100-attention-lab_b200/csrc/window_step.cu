@@ -29,6 +29,7 @@
 // 17 nats below a dominant sink 44 % off).  bf16 terms keep their accuracy at
 // any scale; there the scale is 1 over the number of keys, so that sums of
 // values near the end of fp32's range stay in it, as their average does.
+// Infinite values come out as such: a sum that is not finite is looked over.
 //
 // Measured: 64 sequences, 32 query and 8 key heads of 128, 4100 keys (1.08 GB):
 // 206 us, 5.2 TB/s; without the overlapped fetch 290; with spilled registers
@@ -96,9 +97,53 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
   }
 }
 
+// The visible keys of the token at position p, in order: [0, n_sink) and, from
+// slot0 on around the ring, the window's up to p itself.
+struct Keys {
+  int n, n_sink, slot0;
+  __device__ __forceinline__ Keys(const Params& P, int p) {
+    n_sink = P.sinks <= p ? P.sinks : p + 1;
+    const int w0 = p - P.window + 1 > n_sink ? p - P.window + 1 : n_sink;
+    n = n_sink + (p - w0) + 1;
+    slot0 = w0 < P.cap ? w0 : P.sinks + (w0 - P.sinks) % (P.cap - P.sinks);
+  }
+  __device__ __forceinline__ int slot(const Params& P, int i) const {
+    if (i < n_sink) return i;
+    const int s = slot0 + (i - n_sink);
+    return s < P.cap ? s : s - (P.cap - P.sinks);
+  }
+};
+
+// A warp's sums [rows][D] where they are not finite.  An infinite value times a
+// second term that is 0 or of the other sign is NaN; what its probability, which is
+// above 0, makes of it is the value itself, so the sum of the values that are not
+// finite takes the place of such a sum.  (Works everything out anew: what it
+// took as arguments would cost the kernel's loop registers.)
+template <typename T, int D>
+__device__ __noinline__ void restore_infinities(const Params& P, float* sums, int rows) {
+  const int b = blockIdx.z, hk = blockIdx.y / ((P.G + rows - 1) / rows), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  sums += warp * rows * D;
+  const Keys keys(P, P.positions[b]);
+  const T* vc = static_cast<const T*>(P.vc) + P.vcs[0] * b + P.vcs[2] * hk;
+  const T* vn = static_cast<const T*>(P.v) + P.vs[0] * b + P.vs[1] * hk;
+  const int ntile = (keys.n + 15) / 16, per = (ntile + int(gridDim.x) - 1) / int(gridDim.x);
+  const int first = int(blockIdx.x) * per, end = first + per < ntile ? first + per : ntile;
+  __syncwarp();
+  for (int d = lane; d < D; d += 32) {
+    float total = 0.f;
+    for (int tile = first + warp; tile < end; tile += kWarps)
+      for (int i = tile * 16; i < tile * 16 + 16 && i < keys.n; ++i) {
+        const float v = float((i == keys.n - 1 ? vn : vc + P.vcs[1] * (long long)keys.slot(P, i))[d]);
+        if (!isfinite(v)) total += v;
+      }
+    for (int r = 0; r < rows; ++r)
+      if (total != 0.f && !isfinite(sums[r * D + d])) sums[r * D + d] = total;
+  }
+}
+
 // ROWS query rows (8 or 16) per group; with 8 the lower half of each tile is zero.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kThreads, 2) window_step_kernel(const Params P) {
+__global__ void __launch_bounds__(kThreads, 2) window_step_kernel(const __grid_constant__ Params P) {
   constexpr int KC = D / 32;   // 16-byte pieces of a key per lane
   constexpr int VH = D / 64;   // column halves of V
   constexpr int HR = ROWS / 8;
@@ -122,21 +167,14 @@ __global__ void __launch_bounds__(kThreads, 2) window_step_kernel(const Params P
         reinterpret_cast<uint32_t*>(op + P.os[1] * (i / (D / 2)))[i % (D / 2)] = 0u;
     return;
   }
-  // visible keys in order: [0, n_sink) and [w0, p]
-  const int n_sink = P.sinks <= p ? P.sinks : p + 1;
-  const int w0 = p - P.window + 1 > n_sink ? p - P.window + 1 : n_sink;
-  const int n = n_sink + (p - w0) + 1;
-  const int slot0 = w0 < P.cap ? w0 : P.sinks + (w0 - P.sinks) % (P.cap - P.sinks);
+  const Keys keys(P, p);
+  const int n = keys.n, n_sink = keys.n_sink;
 
   const T* kc = static_cast<const T*>(P.kc) + P.kcs[0] * b + P.kcs[2] * hk;
   const T* vc = static_cast<const T*>(P.vc) + P.vcs[0] * b + P.vcs[2] * hk;
   const T* kn = static_cast<const T*>(P.k) + P.ks[0] * b + P.ks[1] * hk;
   const T* vn = static_cast<const T*>(P.v) + P.vs[0] * b + P.vs[1] * hk;
-  auto slot_of = [&](int i) {
-    if (i < n_sink) return i;
-    const int s = slot0 + (i - n_sink);
-    return s < P.cap ? s : s - (P.cap - P.sinks);
-  };
+  auto slot_of = [&](int i) { return keys.slot(P, i); };
 
   // query fragments, in the keys' order of the inner index
   uint4 qf[HR][KC];
@@ -292,6 +330,9 @@ __global__ void __launch_bounds__(kThreads, 2) window_step_kernel(const Params P
   }
 
   // ---------------------------------------------- join the warps, then the CTAs
+  float odd = 0.f;  // NaN if a sum is not finite
+#pragma unroll
+  for (int i = 0; i < VH * 8 * NC; ++i) odd = fmaf((&acc[0][0][0])[i], 0.f, odd);
 #pragma unroll
   for (int r = 0; r < HR; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -313,6 +354,8 @@ __global__ void __launch_bounds__(kThreads, 2) window_step_kernel(const Params P
               make_float4(acc[c][i][2 * r + e], acc[c][i + 1][2 * r + e], acc[c][i + 2][2 * r + e], acc[c][i + 3][2 * r + e]);
       }
   }
+  if (__any_sync(0xffffffffu, odd != odd))
+    restore_infinities<T, D>(P, s_o, ROWS);
   cluster.sync();
   // every CTA finishes a share of the rows' columns, four at a time
   constexpr int kPiece = D / 4;
