@@ -1,0 +1,59 @@
+"""What the single-token entries leave for others to see: autograd's marks of what they overwrite."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def test_an_overwritten_state_is_noticed_by_autograd():
+    """A state or cache that a recorded graph has saved and a step overwrites: its backward raises."""
+    import gdn_b200
+    B, H, D = 2, 3, 128
+    r = lambda *s: torch.randn(*s, device="cuda")
+
+    def saved(shape, dtype=torch.float32):
+        s = r(*shape).to(dtype).requires_grad_() * 1
+        return s, (s * s).sum()
+
+    x, g = r(B, H, D), -torch.rand(B, H, D, device="cuda")
+    h, loss = saved((B, H, D))
+    with torch.no_grad():
+        gdn_b200.gated_scan_step(x, g, h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+    q = r(B, H, D).bfloat16()
+    s, loss = saved((B, H, D, D))
+    with torch.no_grad():
+        gdn_b200.gdn_step(q, q, q, torch.rand(B, H, device="cuda"), None, s)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+    pos = torch.zeros(B, dtype=torch.int32, device="cuda")
+    for which in range(2):
+        c = [r(B, 9, H, D).bfloat16() for _ in range(2)]
+        c[which], loss = saved((B, 9, H, D), torch.bfloat16)
+        with torch.no_grad():
+            gdn_b200.window_attention_step(q, q, q, *c, pos, 8, 1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_steps_under_inference_mode():
+    """Tensors made there have no version to count; those made before have."""
+    import gdn_b200
+    B, H, D = 1, 2, 128
+    old = torch.zeros(B, H, D, device="cuda")
+    before = old._version
+    with torch.inference_mode():
+        q = torch.randn(B, H, D, device="cuda").bfloat16()
+        beta = torch.rand(B, H, device="cuda")
+        new, S = torch.zeros(B, H, D, device="cuda"), torch.zeros(B, H, D, D, device="cuda")
+        kc, vc = (torch.zeros(B, 4, H, D, device="cuda", dtype=q.dtype) for _ in range(2))
+        for state in (old, new):
+            gdn_b200.gated_scan_step(q, -q.abs(), state)
+        gdn_b200.gdn_step(q, q, q, beta, None, S)
+        gdn_b200.window_attention_step(q, q, q, kc, vc, torch.zeros(B, dtype=torch.int32, device="cuda"), 4)
+        assert torch.equal(old, new)
+    assert old._version > before

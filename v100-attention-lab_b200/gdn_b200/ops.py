@@ -17,6 +17,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd.graph import increment_version  # marks what a kernel has overwritten, as in-place operations do
 
 from . import _lib
 
@@ -371,6 +372,7 @@ def gdn_step(q, k, v, beta, g, state, *, scale=None, output_dtype=None, use_qk_l
         beta.data_ptr(), sb[0], sb[1], 0 if g is None else g.data_ptr(), sg[0], sg[1],
         state.data_ptr(), o.data_ptr(), so[0], so[1])
     _launch(_lib.load().gdn_step_sm100, "gdn_step_sm100", args, dev)
+    increment_version(state)
     return o
 
 

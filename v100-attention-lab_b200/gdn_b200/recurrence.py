@@ -9,6 +9,7 @@ in the sm_100a library through its C ABI.
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .ops import _DTYPES, _check_device, _empty, _launch, _status_ptr
@@ -181,4 +182,5 @@ def gated_scan_step(x, g, state, *, g_activation=None, output_dtype=None):
         x.data_ptr(), sx[0], 0, sx[1], g.data_ptr(), sg[0], 0, sg[1], at, o.data_ptr(), H * D, 0, D, at, 0,
         0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
     _launch(_lib.load().gdn_gated_scan_fwd_sm100, "gdn_gated_scan_fwd_sm100", args, x.device)
+    increment_version(state)
     return o

@@ -12,6 +12,7 @@ from __future__ import annotations
 import operator
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .ops import _DTYPES, _check_device, _empty, _launch, _status_ptr
@@ -172,4 +173,5 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, window, sinks=0,
         k_cache.data_ptr(), skc[0], skc[1], skc[2], v_cache.data_ptr(), svc[0], svc[1], svc[2],
         o.data_ptr(), so[0], so[1], positions.data_ptr())
     _launch(_lib.load().gdn_window_step_sm100, "gdn_window_step_sm100", args, dev)
+    increment_version((k_cache, v_cache))
     return o
