@@ -1,4 +1,4 @@
-"""What the single-token entries leave for others to see: autograd's marks of what they overwrite."""
+"""What autograd is told: of states that are overwritten, and of gradients that are not there."""
 
 import pytest
 import torch
@@ -57,3 +57,13 @@ def test_steps_under_inference_mode():
         gdn_b200.window_attention_step(q, q, q, kc, vc, torch.zeros(B, dtype=torch.int32, device="cuda"), 4)
         assert torch.equal(old, new)
     assert old._version > before
+
+
+def test_a_dual_gradient_is_refused_by_the_backward():
+    """The backward is linear in the outputs' gradient, whose tangent would be dropped without a word."""
+    import gdn_b200
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(1, 20, 1, 8, device="cuda", requires_grad=True)
+    o, _ = gdn_b200.gated_scan(x, -torch.rand_like(x).detach())
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.autograd.grad(o, x, fwd.make_dual(torch.ones_like(o).detach(), torch.ones_like(o).detach()))

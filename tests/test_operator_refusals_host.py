@@ -1,0 +1,41 @@
+"""Requests that the recurrent and windowed operators refuse by name (no GPU needed)."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+import gdn_b200
+
+BF = torch.bfloat16
+
+
+def z(*s, dt=BF):
+    return torch.zeros(*s, dtype=dt)
+
+
+def calls():
+    """Every entry with valid shapes: name, function, tensors."""
+    x, g, h = z(2, 5, 3, 8), z(2, 5, 3, 8, dt=torch.float32), z(2, 3, 8, dt=torch.float32)
+    qkv = [z(1, 4, 4, 64), z(1, 8, 2, 64), z(1, 8, 2, 64)]
+    one = [z(1, 4, 64), z(1, 2, 64), z(1, 2, 64), z(1, 16, 2, 64), z(1, 16, 2, 64)]
+    pos = torch.zeros(1, dtype=torch.int32)
+    gdn = [z(2, 3, 128), z(2, 3, 128), z(2, 3, 128), z(2, 3), z(2, 3), z(2, 3, 128, 128, dt=torch.float32)]
+    return [("gated_scan", gdn_b200.gated_scan, [x, g, h]),
+            ("gated_scan_step", gdn_b200.gated_scan_step, [x[:, 0], g[:, 0], h]),
+            ("window_attention", lambda *t: gdn_b200.window_attention(*t, 4), qkv),
+            ("window_attention_step", lambda *t: gdn_b200.window_attention_step(*t, pos, 8, 4), one),
+            ("gdn_step", gdn_b200.gdn_step, gdn)]
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_forward_mode_gradients_are_refused(which):
+    """A dual tensor's tangent would be dropped without a word."""
+    name, f, tensors = calls()[which]
+    for i, t in enumerate(tensors):
+        with fwd.dual_level():
+            dual = tensors[:i] + [fwd.make_dual(t, torch.ones_like(t))] + tensors[i + 1:]
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    f(*dual)
+            with pytest.raises(ValueError, match="CUDA|one device"):  # no dual among them: the next check
+                f(*tensors)

@@ -17,6 +17,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version  # marks what a kernel has overwritten, as in-place operations do
 
 from . import _lib
@@ -326,6 +327,7 @@ def gdn_step(q, k, v, beta, g, state, *, scale=None, output_dtype=None, use_qk_l
         raise TypeError("q and v must be torch.Tensors")
     if q.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k, v must be [B, H, K] / [B, H, V]")
+    _refuse_tangents("gdn_step", q, k, v, beta, g, state)
     B, H, K = q.shape
     V = v.shape[2]
     dev, dtype, bh = q.device, q.dtype, (B, H)
@@ -410,6 +412,13 @@ def _check_device(name, t, dev, first):
         raise ValueError(f"{name} must be a CUDA tensor (got device {t.device})")
     if t.device != dev:
         raise ValueError(f"{name} is on {t.device}, {first} is on {dev}")
+
+
+def _refuse_tangents(where, *tensors):
+    """Refuse dual tensors: their tangents would be dropped.  (They do not require gradients.)"""
+    if forward_ad._current_level >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{where} has no forward-mode gradient")
 
 
 def _empty(like, dtype):

@@ -12,7 +12,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from .ops import _DTYPES, _check_device, _empty, _launch, _status_ptr
+from .ops import _DTYPES, _check_device, _empty, _launch, _refuse_tangents, _status_ptr
 
 __all__ = ["gated_scan", "gated_scan_step"]
 
@@ -29,6 +29,7 @@ def _check(x, g, state, state_name, output_dtype, dims):
     for name, t in (("x", x), ("g", g), (state_name, state)):
         if not isinstance(t, torch.Tensor) and (t is not None or name != "initial_state"):
             raise TypeError(f"{name} must be a torch.Tensor")
+    _refuse_tangents("the gated recurrence", x, g, state)
     shape, dtype = x.shape, x.dtype
     if len(shape) != len(dims):
         raise ValueError(f"x must be [{', '.join(dims)}] (got shape {tuple(shape)})")
@@ -106,6 +107,7 @@ class _GatedScan(torch.autograd.Function):
 def _backward(ctx, d_o, dht):
     if d_o is None and dht is None:
         return None, None, None, None, None, None
+    _refuse_tangents("the gated recurrence's backward", d_o, dht)
     x, g, states = ctx.saved_tensors
     dev = x.device
     dx, dg = _empty(x, x.dtype), _empty(x, g.dtype)
@@ -137,8 +139,8 @@ def gated_scan(x, g, initial_state=None, *, g_activation=None, output_dtype=None
     Returns:
         (o [B, T, H, D] = every h_t, h_T [B, H, D] fp32 or None)
 
-    The state and all sums are fp32.  Differentiable (once) in x, g and
-    initial_state; the backward recomputes the states in fp32 from x and g and
+    The state and all sums are fp32.  Differentiable (once, in reverse mode) in
+    x, g and initial_state; the backward recomputes the states in fp32 from x and g and
     states kept every 64 (fp32 x) or 128 rows.  Results repeat bit for bit.
     Launches on the current stream of x's device without synchronising.
     """

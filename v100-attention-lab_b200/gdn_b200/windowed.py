@@ -15,7 +15,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from .ops import _DTYPES, _check_device, _empty, _launch, _status_ptr
+from .ops import _DTYPES, _check_device, _empty, _launch, _refuse_tangents, _status_ptr
 
 __all__ = ["window_attention", "window_attention_step"]
 
@@ -35,6 +35,7 @@ def _check_tensors(tensors):
             raise ValueError(f"{name} must have a contiguous last dimension")
         if grad and t.requires_grad:
             raise NotImplementedError("windowed attention has no backward: call it under torch.no_grad()")
+    _refuse_tangents("windowed attention", *(t for _, t in tensors))
     if dtype != torch.bfloat16 and dtype != torch.float16:
         raise NotImplementedError(f"gdn_b200 takes fp16 or bf16 q/k/v (got {dtype})")
 
