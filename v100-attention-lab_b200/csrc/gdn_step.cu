@@ -137,8 +137,9 @@ int validate(const gdn_step_args* a) {
   const int64_t* st[3] = {a->q_stride, a->k_stride, a->v_stride};
   for (int i = 0; i < 3; ++i) {
     if (reinterpret_cast<uintptr_t>(ptr[i]) % 8) return GDN_ERR_ALIGNMENT;
+    // a dimension of one element may come with any stride: it is never taken
     for (int j = 0; j < 2; ++j)
-      if (st[i][j] < 0 || st[i][j] % 4) return GDN_ERR_ALIGNMENT;
+      if ((j == 0 ? a->B : a->H) > 1 && (st[i][j] < 0 || st[i][j] % 4)) return GDN_ERR_ALIGNMENT;
   }
   if (reinterpret_cast<uintptr_t>(a->o) % size_t(dtype_size(a->out_dtype))) return GDN_ERR_ALIGNMENT;
   for (int j = 0; j < 2; ++j)
