@@ -38,7 +38,7 @@ enum gdn_status {
   GDN_OK = 0,
   GDN_ERR_INVALID_ARGUMENT = 1, /* bad pointer, shape, stride or dtype       */
   GDN_ERR_UNSUPPORTED = 2,      /* valid request this build does not handle  */
-  GDN_ERR_ALIGNMENT = 3,        /* base/stride not 16-byte aligned (TMA)     */
+  GDN_ERR_ALIGNMENT = 3,        /* base/stride not aligned as the entry needs */
   GDN_ERR_CUDA = 4,             /* a CUDA runtime call failed                */
   GDN_ERR_TIMEOUT = 5,          /* a device-side bounded wait expired        */
   GDN_ERR_NO_DEVICE = 6,        /* no sm_100 device is current               */
@@ -316,8 +316,8 @@ int gdn_window_step_sm100(const gdn_window_step_args* args, void* stream);
  *   q, k [B, H, K]   v [B, H, V]   in_dtype (fp16 or bf16, last dim contiguous,
  *   8-byte aligned rows);  beta, g [B, H] float32, g may be NULL (g == 0);
  *   o [B, H, V] out_dtype
- * Strides in elements for (b, h); flags and scale as in gdn_fwd_args, without
- * the solver flags.
+ * Strides in elements for (b, h), any for a dimension of one element; flags and
+ * scale as in gdn_fwd_args, without the solver flags.
  */
 typedef struct gdn_step_args {
   int32_t abi_version; /* must be GDN_B200_ABI_VERSION */

@@ -39,3 +39,10 @@ def test_forward_mode_gradients_are_refused(which):
                     f(*dual)
             with pytest.raises(ValueError, match="CUDA|one device"):  # no dual among them: the next check
                 f(*tensors)
+
+
+def test_the_alignment_status_names_the_entries_rules():
+    from gdn_b200 import _build, _lib
+    _build.build()
+    text = _lib.status_string(_lib.ERR_ALIGNMENT)
+    assert "16-byte" in text and "gdn_step: 8-byte" in text and "gated_scan: whole elements" in text

@@ -947,7 +947,7 @@ extern "C" const char* gdn_status_string(int code) {
     case GDN_OK: return "ok";
     case GDN_ERR_INVALID_ARGUMENT: return "invalid argument (pointer, shape, stride or dtype)";
     case GDN_ERR_UNSUPPORTED: return "unsupported configuration (GDN: K=V=128, chunk_size=64, fp16/bf16; other entry points: see gdn_b200.h)";
-    case GDN_ERR_ALIGNMENT: return "tensor base or stride is not 16-byte aligned";
+    case GDN_ERR_ALIGNMENT: return "tensor base or stride is not aligned (16-byte rows; gdn_step: 8-byte rows; gated_scan: whole elements)";
     case GDN_ERR_CUDA: return "CUDA runtime error";
     case GDN_ERR_TIMEOUT: return "device-side wait timed out (kernel aborted)";
     case GDN_ERR_NO_DEVICE: return "current device is not sm_100 (B200)";
