@@ -252,6 +252,7 @@ uint64_t gdn_gated_scan_states_bytes(const gdn_gated_scan_args* args);
  *         T <= S, H a multiple of HK (query head h reads key head h / (H / HK))
  *   lengths  [B] int32 on the device, clamped to 0..S, or NULL (all S)
  * Strides in elements for (batch, row, head); bases and strides 16-byte aligned.
+ * q, k and v may have a stride of 0 over the batch or the heads (expanded).
  */
 typedef struct gdn_window_attn_args {
   int32_t abi_version; /* must be GDN_B200_ABI_VERSION */

@@ -46,3 +46,12 @@ def test_the_alignment_status_names_the_entries_rules():
     _build.build()
     text = _lib.status_string(_lib.ERR_ALIGNMENT)
     assert "16-byte" in text and "gdn_step: 8-byte" in text and "gated_scan: whole elements" in text
+
+
+def test_expanded_rows_are_refused():
+    q, k, v = calls()[2][2]
+    for i, name in enumerate("qkv"):
+        t = [q, k, v]
+        t[i] = t[i][:, :1].expand(t[i].shape)
+        with pytest.raises(ValueError, match=f"{name} .*expanded"):
+            gdn_b200.window_attention(*t, 4)

@@ -74,6 +74,7 @@ struct Params {
   void* o;
   int* status;
   long long so_b, so_t, so_h;
+  int qb, qh, kb, kh, vb, vh;  // 0 where an input is expanded over the batch or the heads (one element of the map), else 1
   int T, S, HK, G;
   int window, sinks;
   int nx, ny, items;  // row tiles (or pairs) and heads (or pairs) of an item grid, items in all
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
               mbar_arrive_expect_tx(&bars[B_Q + x], L::qtile);
               for (uint32_t c = 0; c < L::boxes; ++c)
                 tma_load_4d(sm + L::q + x * L::qtile + c * 16384, &P.tm_q, &bars[B_Q + x], c * 64, it.row(P, x),
-                            it.head(P, x), it.b);
+                            it.head(P, x) * P.qh, it.b * P.qb);
             }
             __syncwarp();
             ++nq;
@@ -457,8 +458,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
               const bool v = u >= 0, k = u + 2 < it.count;
               mbar_arrive_expect_tx(&full[s], (v + k) * L::kvtile);
               for (uint32_t c = 0; c < L::boxes; ++c) {
-                if (v) tma_load_4d(dst + c * 8192, &P.tm_v, &full[s], c * 64, it.key0(u), it.hk, it.b);
-                if (k) tma_load_4d(dst + L::kvtile + c * 8192, &P.tm_k, &full[s], c * 64, it.key0(u + 2), it.hk, it.b);
+                if (v) tma_load_4d(dst + c * 8192, &P.tm_v, &full[s], c * 64, it.key0(u), it.hk * P.vh, it.b * P.vb);
+                if (k)
+                  tma_load_4d(dst + L::kvtile + c * 8192, &P.tm_k, &full[s], c * 64, it.key0(u + 2), it.hk * P.kh,
+                              it.b * P.kb);
               }
             }
             __syncwarp();
@@ -766,8 +769,9 @@ int validate(const gdn_window_attn_args* a) {
   for (int i = 0; i < 4; ++i) {
     if (reinterpret_cast<uintptr_t>(ptr[i]) % 16) return GDN_ERR_ALIGNMENT;
     const int n[3] = {a->B, i == 1 || i == 2 ? a->S : a->T, i == 1 || i == 2 ? a->HK : a->H};
+    // stride 0: an input that is expanded over the batch or the heads
     for (int j = 0; j < 3; ++j)
-      if (n[j] > 1 && (st[i][j] <= 0 || st[i][j] % 8 != 0)) return GDN_ERR_ALIGNMENT;
+      if (n[j] > 1 && (st[i][j] < 0 || st[i][j] % 8 != 0 || (st[i][j] == 0 && (i == 3 || j == 1)))) return GDN_ERR_ALIGNMENT;
   }
   if (reinterpret_cast<uintptr_t>(a->lengths) % 4) return GDN_ERR_ALIGNMENT;
   return GDN_OK;
@@ -777,9 +781,10 @@ bool make_map(CUtensorMap* m, const gdn_window_attn_args* a, const void* base, c
               int box_rows) {
   const CUtensorMapDataType dt =
       a->dtype == GDN_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const uint64_t dims[4] = {uint64_t(a->D), uint64_t(rows), uint64_t(heads), uint64_t(a->B)};
-  // a dimension of one element may come with any stride: it is never taken
-  auto bytes = [&](int64_t s, int n) { return n > 1 ? uint64_t(s) * 2 : uint64_t(a->D) * 2; };
+  // a dimension of stride 0 is one element
+  const uint64_t dims[4] = {uint64_t(a->D), uint64_t(rows), st[2] != 0 ? uint64_t(heads) : 1, st[0] != 0 ? uint64_t(a->B) : 1};
+  // and one of one element may come with any stride: it is never taken
+  auto bytes = [&](int64_t s, int n) { return n > 1 && s != 0 ? uint64_t(s) * 2 : uint64_t(a->D) * 2; };
   const uint64_t strides[3] = {bytes(st[1], rows), bytes(st[2], heads), bytes(st[0], a->B)};
   const uint32_t box[4] = {64, uint32_t(box_rows), 1, 1};
   return make_tmap(m, dt, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -812,6 +817,10 @@ int run(const gdn_window_attn_args* a, void* stream) {
   p.o = a->o;
   p.status = a->status;
   p.so_b = a->o_stride[0], p.so_t = a->o_stride[1], p.so_h = a->o_stride[2];
+  auto steps = [](int64_t stride) { return stride != 0 ? 1 : 0; };
+  p.qb = steps(a->q_stride[0]), p.qh = steps(a->q_stride[2]);
+  p.kb = steps(a->k_stride[0]), p.kh = steps(a->k_stride[2]);
+  p.vb = steps(a->v_stride[0]), p.vh = steps(a->v_stride[2]);
   p.T = a->T, p.S = a->S, p.HK = a->HK, p.G = a->H / a->HK;
   // a window or sinks past the keys see no more than all of them
   p.window = a->window < a->S ? a->window : a->S;

@@ -73,7 +73,8 @@ def window_attention(q, k, v, window, sinks=0, *, scale=None, lengths=None):
         q: [B, T, H, D] fp16/bf16, D 64 or 128 (last dim contiguous, rows
             16-byte aligned)
         k, v: [B, S, HK, D] same dtype, S >= T, H a multiple of HK: query head
-            h reads key head h // (H // HK)
+            h reads key head h // (H // HK); like q they may be expanded
+            (stride 0) over the batch or the heads
         window: tokens a row sees, itself included (>= 1)
         sinks: first tokens that stay visible behind the window
         scale: factor of q k^T, positive; None = 1/sqrt(D)
@@ -101,6 +102,10 @@ def window_attention(q, k, v, window, sinks=0, *, scale=None, lengths=None):
         raise ValueError(f"the number of query heads ({H}) must be a multiple of the key heads ({HK})")
     if S < T:
         raise ValueError(f"fewer keys ({S}) than query rows ({T})")
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    if (sq[1] == 0 and T > 1) or ((sk[1] == 0 or sv[1] == 0) and S > 1):
+        name = "q" if sq[1] == 0 and T > 1 else "k" if sk[1] == 0 else "v"
+        raise ValueError(f"{name} must not be expanded along its rows (stride 0); over the batch or the heads it may be")
     window, sinks = operator.index(window), operator.index(sinks)
     scale = _check_sizes(D, window, sinks, scale)
     dev = q.device
@@ -109,7 +114,7 @@ def window_attention(q, k, v, window, sinks=0, *, scale=None, lengths=None):
         _check_device("lengths", lengths, dev, "q")
     _check_devices(tensors, dev)
     o = _empty(q, q.dtype)
-    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), o.stride()
+    so = o.stride()
     args = _lib.WINDOW_ATTN_ARGS.pack(
         # beyond the keys neither window nor sinks change anything
         _lib.ABI_VERSION, B, T, S, H, HK, D, _DTYPES[q.dtype], min(window, S), min(sinks, S), scale, 0,
