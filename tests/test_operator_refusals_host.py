@@ -55,3 +55,11 @@ def test_expanded_rows_are_refused():
         t[i] = t[i][:, :1].expand(t[i].shape)
         with pytest.raises(ValueError, match=f"{name} .*expanded"):
             gdn_b200.window_attention(*t, 4)
+
+
+def test_a_scale_of_zero_is_refused():
+    """0 stands for "not given" in the C structs, so the call would answer with a scale of 1."""
+    t = calls()[4][2]
+    for scale in (0.0, 0, -0.0):
+        with pytest.raises(ValueError, match="scale"):
+            gdn_b200.gdn_step(*t, scale=scale)

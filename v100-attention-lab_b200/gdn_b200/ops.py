@@ -315,7 +315,7 @@ def gdn_step(q, k, v, beta, g, state, *, scale=None, output_dtype=None, use_qk_l
         beta, g: [B, H], cast to fp32 if needed; g is the log decay, None = 0
         state: [B, H, V, K] fp32, contiguous; overwritten with the new state
         scale, use_qk_l2norm_in_kernel, beta_activation, g_activation: as in
-            ``gdn_chunk_fwd``
+            ``gdn_chunk_fwd`` (scale not 0)
         output_dtype: dtype of o (default q.dtype)
     Returns:
         o [B, H, V]
@@ -358,6 +358,9 @@ def gdn_step(q, k, v, beta, g, state, *, scale=None, output_dtype=None, use_qk_l
     flags = _prep_flags(use_qk_l2norm_in_kernel, beta_activation, g_activation)
     if g is None and g_activation is not None:
         raise ValueError("g_activation needs a g tensor")
+    scale = 1.0 if scale is None else float(scale)
+    if scale == 0.0:  # the C struct's "not given"
+        raise ValueError("scale must not be 0")
     if not q.is_cuda:
         raise ValueError(f"q must be a CUDA tensor (got device {dev})")
     if k.device != dev or v.device != dev or beta.device != dev or state.device != dev or (g is not None and g.device != dev):
@@ -369,7 +372,7 @@ def gdn_step(q, k, v, beta, g, state, *, scale=None, output_dtype=None, use_qk_l
     o = _empty(v, out_dtype)
     sb, sg, so = beta.stride(), (0, 0) if g is None else g.stride(), o.stride()
     args = _lib.STEP_ARGS.pack(
-        _lib.ABI_VERSION, B, H, K, V, _DTYPES[dtype], _DTYPES[out_dtype], flags, 1.0 if scale is None else float(scale), 0,
+        _lib.ABI_VERSION, B, H, K, V, _DTYPES[dtype], _DTYPES[out_dtype], flags, scale, 0,
         q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1],
         beta.data_ptr(), sb[0], sb[1], 0 if g is None else g.data_ptr(), sg[0], sg[1],
         state.data_ptr(), o.data_ptr(), so[0], so[1])
