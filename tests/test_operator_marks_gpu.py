@@ -1,4 +1,4 @@
-"""What autograd is told: of states that are overwritten, and of gradients that are not there."""
+"""What autograd is told (of states that are overwritten, of gradients that are not there), and captured tokens."""
 
 import pytest
 import torch
@@ -67,3 +67,36 @@ def test_a_dual_gradient_is_refused_by_the_backward():
     o, _ = gdn_b200.gated_scan(x, -torch.rand_like(x).detach())
     with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         torch.autograd.grad(o, x, fwd.make_dual(torch.ones_like(o).detach(), torch.ones_like(o).detach()))
+
+
+def test_captured_tokens_of_the_recurrences():
+    """One captured token of gdn_step and gated_scan_step, replayed along a sequence."""
+    import gdn_b200
+    B, H, D, n = 2, 3, 128, 12
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=gen)
+    q, k, v = (torch.nn.functional.normalize(r(n, B, H, D), dim=-1).bfloat16() for _ in range(3))
+    beta, g, z = r(n, B, H), r(n, B, H) + 2, r(n, B, H, D) + 2
+    kw = dict(beta_activation="sigmoid", g_activation="logsigmoid")
+    S0, h0 = 0.1 * r(B, H, D, D), r(B, H, D)
+
+    def token(i, S, h):
+        return (gdn_b200.gdn_step(i[0], i[1], i[2], i[3], i[4], S, **kw),
+                gdn_b200.gated_scan_step(i[2], i[5], h, g_activation="logsigmoid"))
+
+    rows = [[t[j] for t in (q, k, v, beta, g, z)] for j in range(n)]
+    S, h = S0.clone(), h0.clone()
+    want = [token(i, S, h) for i in rows]
+    slots = [torch.zeros_like(t) for t in rows[0]]
+    Sg, hg = S0.clone(), h0.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = token(slots, Sg, hg)
+    Sg.copy_(S0), hg.copy_(h0)
+    for j in range(n):
+        for s, t in zip(slots, rows[j]):
+            s.copy_(t)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[j])), j
+    assert torch.equal(Sg, S) and torch.equal(hg, h)
