@@ -63,3 +63,10 @@ def test_a_scale_of_zero_is_refused():
     for scale in (0.0, 0, -0.0):
         with pytest.raises(ValueError, match="scale"):
             gdn_b200.gdn_step(*t, scale=scale)
+
+
+@pytest.mark.parametrize("scale", [1e-50, -1e-46, 1e39, float("inf"), -float("inf"), float("nan")])
+def test_scales_outside_fp32_are_refused(scale):
+    """1e-50 would be packed as 0, which stands for 1; 1e39 would raise OverflowError."""
+    with pytest.raises(ValueError, match="scale"):
+        gdn_b200.gdn_step(*calls()[4][2], scale=scale)

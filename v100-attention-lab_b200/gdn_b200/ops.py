@@ -359,8 +359,8 @@ def gdn_step(q, k, v, beta, g, state, *, scale=None, output_dtype=None, use_qk_l
     if g is None and g_activation is not None:
         raise ValueError("g_activation needs a g tensor")
     scale = 1.0 if scale is None else float(scale)
-    if scale == 0.0:  # the C struct's "not given"
-        raise ValueError("scale must not be 0")
+    if not 1e-45 < abs(scale) < 3e38:  # an fp32 number; 0 is the C struct's "not given"
+        raise ValueError(f"scale must be finite and not 0 (got {scale})")
     if not q.is_cuda:
         raise ValueError(f"q must be a CUDA tensor (got device {dev})")
     if k.device != dev or v.device != dev or beta.device != dev or state.device != dev or (g is not None and g.device != dev):
