@@ -148,3 +148,25 @@ def test_infinities_that_one_token_sees(dt, size):
     assert (got[..., 5] == inf).all() and (got[..., 9] == inf).all()
     assert (got[..., 6] == -inf).all()
     assert got[..., [7, 8, 21]].isnan().all()
+
+
+def test_scores_that_are_not_finite_one_token():
+    """A NaN or infinite query or key makes NaN of the heads that meet it, and of no others."""
+    import gdn_b200
+    B, H, HK, D, window, sinks = 2, 40, 2, 64, 300, 2
+    cap = window + sinks
+    q, k, v = make(B, 1, 1, H, HK, D, torch.bfloat16, 8)
+    kc, vc = make(B, cap, cap, HK, HK, D, torch.bfloat16, 9)[1:]
+    pos = torch.full((B,), cap - 1, dtype=torch.int32, device="cuda")
+    clean = gdn_b200.window_attention_step(q[:, 0], k[:, 0], v[:, 0], kc, vc, pos, window, sinks)
+    q[0, 0, 3], q[0, 0, 18, 5] = float("nan"), float("nan")  # two heads of key head 0, in either group of 16
+    kc[1, 150, 1, 7] = float("nan")                           # all heads of key head 1
+    vc[0, 100, 0, 9] = float("inf")
+    o = gdn_b200.window_attention_step(q[:, 0], k[:, 0], v[:, 0], kc, vc, pos, window, sinks)
+    bad = torch.zeros(B, H, dtype=torch.bool, device="cuda")
+    bad[0, 3] = bad[0, 18] = True
+    bad[1, 20:] = True
+    assert o[bad].isnan().all()
+    want = clean.clone()
+    want[0, :20, 9] = float("inf")
+    assert torch.equal(o[~bad], want[~bad])

@@ -122,23 +122,47 @@ struct Keys {
 template <typename T, int D>
 __device__ __noinline__ void restore_infinities(const Params& P, float* sums, int rows) {
   const int b = blockIdx.z, hk = blockIdx.y / ((P.G + rows - 1) / rows), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // rows whose sum of probabilities is not finite come out as NaN in any case
+  const float* l = sums + kWarps * rows * (D + 1) + warp * rows;
+  const int real = P.G - (blockIdx.y - hk * ((P.G + rows - 1) / rows)) * rows;
+  bool any = false;
+  __syncwarp();
+  for (int r = 0; r < rows && r < real; ++r) any |= isfinite(l[r]);
+  if (!any) return;
   sums += warp * rows * D;
   const Keys keys(P, P.positions[b]);
   const T* vc = static_cast<const T*>(P.vc) + P.vcs[0] * b + P.vcs[2] * hk;
   const T* vn = static_cast<const T*>(P.v) + P.vs[0] * b + P.vs[1] * hk;
   const int ntile = (keys.n + 15) / 16, per = (ntile + int(gridDim.x) - 1) / int(gridDim.x);
   const int first = int(blockIdx.x) * per, end = first + per < ntile ? first + per : ntile;
-  __syncwarp();
-  for (int d = lane; d < D; d += 32) {
-    float total = 0.f;
-    for (int tile = first + warp; tile < end; tile += kWarps)
-      for (int i = tile * 16; i < tile * 16 + 16 && i < keys.n; ++i) {
-        const float v = float((i == keys.n - 1 ? vn : vc + P.vcs[1] * (long long)keys.slot(P, i))[d]);
-        if (!isfinite(v)) total += v;
+  constexpr int N = D / 32;  // columns of a lane, 2 or 4
+  float total[N];
+#pragma unroll
+  for (int c = 0; c < N; ++c) total[c] = 0.f;
+  for (int tile = first + warp; tile < end; tile += kWarps) {
+    uint32_t v[16][N / 2];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int i = tile * 16 + j < keys.n ? tile * 16 + j : keys.n - 1;  // the last key twice: no other sum
+      const T* src = (i == keys.n - 1 ? vn : vc + P.vcs[1] * (long long)keys.slot(P, i)) + lane * N;
+#pragma unroll
+      for (int c = 0; c < N / 2; ++c) v[j][c] = reinterpret_cast<const uint32_t*>(src)[c];
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int c = 0; c < N / 2; ++c) {
+        const float2 x = Cvt<T>::unpack(v[j][c]);
+        if (!isfinite(x.x)) total[2 * c] += x.x;
+        if (!isfinite(x.y)) total[2 * c + 1] += x.y;
       }
-    for (int r = 0; r < rows; ++r)
-      if (total != 0.f && !isfinite(sums[r * D + d])) sums[r * D + d] = total;
   }
+  for (int r = 0; r < rows; ++r)
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      float* s = sums + r * D + lane * N + c;
+      if (total[c] != 0.f && !isfinite(*s)) *s = total[c];
+    }
 }
 
 // ROWS query rows (8 or 16) per group; with 8 the lower half of each tile is zero.
