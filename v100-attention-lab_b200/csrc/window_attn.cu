@@ -23,12 +23,18 @@
 // columns and are the second product's TMEM operand, so they never touch shared
 // memory.
 //
-// What was tried: 128-key tiles with one score buffer leave the softmax waiting
-// for both products (1119 us at 16384 tokens, 32 query and 8 key heads of 128,
-// window 4096, against 851); two threads per row, to have more warps to switch
-// between, cost more instructions than they hide (922); a quarter of the
-// exponentials as polynomials on the FMA pipe gain nothing (868).  A spilled
-// register costs dearly: with this much shared memory taken, local memory is L2.
+// Measured, 16384 tokens, 32 query and 8 key heads of 128, window 4096, fp16: 842 us
+// on the GPU alone (a few launches of a replayed graph), 970 to 990 a call under
+// lasting load, where the clock gives way; with heads of 64 684 and 759.  2 x 4096
+// tokens, 16 heads of 128, window 1024: 80 and 90.
+//
+// What was tried, GPU alone, each against the build of its day: two threads per row,
+// to have more warps to switch between, together with a quarter of the
+// exponentials as polynomials on the FMA pipe, 922, and 851 without either; the polynomials
+// with one thread per row 868.  64-key tiles with two score buffers came in one
+// step with the cheap MMA issue below (1119 -> 1006): what the tile's size does by
+// itself is not known.  A spilled register costs dearly: with this much shared
+// memory taken, local memory is L2.
 //
 // The probabilities are rounded once to the operands' type, as the 16-bit product
 // has to have them.  Where keys of like weight make up the output that adds as
@@ -167,15 +173,16 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 
 // How far (log2) a row's probabilities may pass 1 before its reference follows
 // the maximum, and the scale that they get before they are rounded, which the sum
-// shares, so that it cancels.  fp16 has a grid of 2^-24 and ends at 2^16: with the
-// reference at 2^11 a probability is exact to 2^-36, or to its own half step (at
-// 1, with a slack of 8, keys 15 nats below a dominant sink were 8 half steps off
-// and those 18 below it lost); a factor of 2 is left for the exponent's rounding at
-// scores of millions.  A smaller slack has O scaled more often: a call of 1x16384
-// tokens, 32/8 heads of 128, window 4096, takes 985 to 996 us at 8 and at 4 alike,
-// 1013 at 3, 1071 at 2.  bf16 keeps its accuracy at any scale: it takes the slack and the number of
-// keys back, so that sums of values near the end of fp32's range stay in it, as
-// their average does.
+// shares, so that it cancels.
+// fp16 has a grid of 2^-24 and ends at 2^16: with the reference at 2^11 a
+// probability is exact to 2^-36, or to its own half step (at 1, with a slack of 8,
+// keys 15 nats below a dominant sink were 8 half steps off and those 18 below it
+// lost); a factor of 2 is left for the exponent's rounding at scores of millions.
+// A smaller slack has O scaled more often: a call of 1 x 16384 tokens, 32/8 heads of
+// 128, window 4096, takes 985 to 996 us at 8 and at 4 alike, 1013 at 3, 1071 at 2.
+// bf16 keeps its accuracy at any scale: it takes the slack and the number of keys
+// back, so that sums of values near the end of fp32's range stay in it, as their
+// average does (values below some 2^-100 lose bits instead).
 template <typename T> constexpr float kSlack = Cvt<T>::kIsBf16 ? 8.f : 4.f;
 float shift_of(int dtype, long long keys) {
   return dtype == GDN_DTYPE_F16 ? 11.f : -kSlack<__nv_bfloat16> - float(std::ceil(std::log2(double(keys))));
@@ -226,7 +233,7 @@ template <> struct Pair<__nv_bfloat16> {
 // One of a work item's two query tiles: which rows it has and which keys they see.
 struct Rows {
   int p0, p1;  // positions of its first row and of its last one that exists (p1 < p0: no rows)
-  int len, window, sinks;
+  int len, window;
 
   // whether it has a row that sees anything (then its first row sees itself)
   __device__ __forceinline__ bool used() const { return p1 >= p0 && p0 < len; }
@@ -263,7 +270,7 @@ struct Item {
   __device__ __forceinline__ Rows rows(const Params& P, int x) const {
     const int r = row(P, x);
     const int p0 = P.S - P.T + r;
-    return Rows{p0, x && P.single ? p0 - 1 : P.S - P.T + (r + kTile < P.T ? r + kTile : P.T) - 1, len, P.window, P.sinks};
+    return Rows{p0, x && P.single ? p0 - 1 : P.S - P.T + (r + kTile < P.T ? r + kTile : P.T) - 1, len, P.window};
   }
 };
 
@@ -430,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     bool careful = false;
     do {
       if (warp == kTmaWarp) {
-        // -------------------------------------------- producer: Q tiles, then K0 V0 K1 V1 ...
+        // -------------------------------------------- producer: Q tiles, then the ring's stages, V of tile u and K of u + 2
         for (int j = 0, i = blockIdx.x; i < P.items && ok; ++j, i += gridDim.x) {
           if (careful && !(redo[j >> 5] >> (j & 31) & 1)) continue;
           const Item it = make_item(P, i);
