@@ -247,7 +247,8 @@ uint64_t gdn_gated_scan_states_bytes(const gdn_gated_scan_args* args);
  *     j <= p,  j < lengths[b],  and  (p - j < window  or  j < sinks).
  * o = softmax(scale q k^T) v over the visible keys; 0 where there are none
  * (rows at or behind their sequence's length).  Hidden keys and values may hold
- * anything, NaN and infinities included.
+ * anything, NaN and infinities included.  A visible infinite value gives an
+ * infinity, or NaN where its probability rounds to 0 (fp16: 2^-36 of the largest).
  *   q, o  [B, T, H, D]   k, v  [B, S, HK, D]   fp16 or bf16, D = 64 or 128,
  *         T <= S, H a multiple of HK (query head h reads key head h / (H / HK))
  *   lengths  [B] int32 on the device, clamped to 0..S, or NULL (all S)
